@@ -162,7 +162,7 @@ DEV float gelu_grad(float x) {
   return 0.5f * (1.f + erff(x * 0.70710678118654752f)) + x * 0.39894228040143268f * __expf(-0.5f * x * x);
 }
 // erf-form GELU on two values at once, erf from Abramowitz & Stegun 7.1.26 (|error| <= 1.5e-7,
-// far below the bf16 rounding of the result): packed-math polynomial (v_pk_fma_f32), native
+// far below the bf16 rounding of the result): polynomial on both at once, native
 // v_rcp_f32 / v_exp_f32 -- roughly a third of the instructions of two library erff calls
 DEV f32x2 gelu_fast2(f32x2 x) {
   const f32x2 u = f32x2{fabsf(x[0]), fabsf(x[1])} * 0.70710678118654752f;
