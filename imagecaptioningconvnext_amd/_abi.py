@@ -54,6 +54,20 @@ class MhaDesc(ctypes.Structure):
         ("probs", c_void_p)]
 
 
+class PagedWriteDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "n", "heads", "dh", "page", "pages")] + [
+        (n, c_int64) for n in ("k_row", "k_head", "v_row", "v_head", "kc_page", "kc_tok", "kc_head", "vc_page",
+                               "vc_tok", "vc_head")] + [(n, c_void_p) for n in ("k", "v", "kc", "vc", "slots")]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "B", "H", "Hkv", "dh", "page", "pages", "width",
+                                              "max_len")] + [("scale", c_float)] + [
+        (n, c_int64) for n in ("q_row", "q_head", "o_row", "o_head", "k_page", "k_tok", "k_head", "v_page", "v_tok",
+                               "v_head", "table_row")] + [
+        (n, c_void_p) for n in ("q", "k", "v", "o", "lse", "table", "lens", "ws")] + [("ws_bytes", c_int64)]
+
+
 class GemmProblem(ctypes.Structure):
     _fields_ = [("A", c_void_p), ("B", c_void_p), ("C", c_void_p), ("lda", c_int64), ("ldb", c_int64),
                 ("ldc", c_int64), ("M", ctypes.c_int32), ("N", ctypes.c_int32), ("K", ctypes.c_int32),
@@ -140,12 +154,18 @@ _SIGS = {
                              c_void_p],
     "imgcap_greedy_select": [c_int, c_int, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_void_p, c_void_p,
                              c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
+    "imgcap_paged_plan": [c_int] * 5 + [c_void_p] * 3 + [c_int64] + [c_void_p] * 11,
+    "imgcap_paged_write": [ctypes.POINTER(PagedWriteDesc), c_void_p],
+    "imgcap_paged_attention_ws": [ctypes.POINTER(PagedAttnDesc), ctypes.POINTER(c_int64)],
+    "imgcap_paged_attention": [ctypes.POINTER(PagedAttnDesc), c_void_p],
+    "imgcap_token_logprobs": [c_int] * 4 + [c_void_p, c_int64] + [c_void_p] * 7,
+    "imgcap_token_logprobs_bwd": [c_int] * 3 + [c_void_p, c_int64] + [c_void_p] * 6 + [c_int64, c_void_p],
     "imgcap_slice_reduce": [c_int64, c_int, c_void_p, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p],
 }
 
 _lib = None
 # include/imgcap_abi.h IMGCAP_ABI_VERSION (tests/test_abi_cpu.py checks the two agree)
-ABI_VERSION = 6
+ABI_VERSION = 7
 
 
 def lib():
@@ -200,6 +220,14 @@ def _grow_workspaces(dev):
         lib().imgcap_workspace_needed(slot, ctypes.byref(need))
         if need.value > _ws[(dev, slot)].numel():
             _attach(dev, slot, need.value * 5 // 4)
+
+
+def check(name, *args):
+    """Call an entry point that only computes on the host (no workspace is attached for it)."""
+    rc = getattr(lib(), name)(*args)
+    if rc != 0:
+        msg = lib().imgcap_last_error_string().decode(errors="replace")
+        raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
 
 
 def call(name, *args):

@@ -1,0 +1,576 @@
+// Paged key/value cache of incremental decoding: page planning from the requests' lengths, the
+// writer of new tokens' keys and values, and attention of one new token per request.
+//
+// A cache is [pages][page][kv heads][dh] (any strides, unit inner one); a request owns the pages
+// that its row of the table names, position p of it sits in slot table[p / page] * page + p % page.
+#include "common.h"
+
+namespace imgcap {
+
+// ---- page planning ------------------------------------------------------------------------
+// One workgroup walks the requests in chunks of its width: integer prefix sums give each request
+// its place on the stack of free pages and its first token, then every token finds its request by
+// bisection of the starts.  All sums are 64-bit: lengths are the caller's and may be anything.
+DEV long wave_scan_incl(long v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long u = __shfl_up(v, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) v += u;
+  }
+  return v;
+}
+// inclusive prefix over the block; `total` gets the block's sum.  red: blockDim / 64 longs.
+DEV long block_scan_incl(long v, long* red, long& total) {
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  v = wave_scan_incl(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) red[w] = v;
+  __syncthreads();
+  long before = 0, all = 0;
+  for (int i = 0; i < nw; ++i) {
+    if (i < w) before += red[i];
+    all += red[i];
+  }
+  total = all;
+  return v + before;
+}
+
+struct PlanArgs {
+  int B, width, lp, pool, tokens;
+  const int32_t* past;
+  const int32_t* add;
+  int32_t* table;
+  long table_row;
+  int32_t* free_ids;
+  const int32_t* count;
+  int32_t* count_out;
+  int32_t* lens;
+  int32_t* starts;
+  int64_t* slots;
+  int32_t* rows;
+  int64_t* positions;
+  int32_t* waits;
+  int32_t* ws;  // [B] first page of each request on the stack, [B] = the stack's top
+};
+
+// token i of the step: its request, position and slot; the token that opens a page enters the page
+// into the table
+DEV void plan_token(const PlanArgs& a, int i, int total, const int32_t* starts, const int32_t* first, int top) {
+  if (i >= total) {
+    a.slots[i] = -1;
+    a.rows[i] = -1;
+    a.positions[i] = 0;
+    return;
+  }
+  int lo = 0, hi = a.B;  // starts[lo] <= i < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= i) lo = mid;
+    else hi = mid;
+  }
+  const int past = a.past[lo], page = 1 << a.lp;
+  const long pos = (long)past + (i - starts[lo]);
+  const int pi = (int)(pos >> a.lp), off = (int)pos & (page - 1);
+  const int have = (int)(((long)past + page - 1) >> a.lp);
+  int32_t* entry = a.table + (long)lo * a.table_row + pi;
+  int id;
+  if (pi < have) {
+    id = *entry;
+  } else {
+    id = a.free_ids[top - 1 - first[lo] - (pi - have)];
+    if (off == 0) *entry = id;
+  }
+  a.slots[i] = (unsigned)id < (unsigned)a.pool ? ((int64_t)id << a.lp) + off : -1;
+  a.rows[i] = lo;
+  a.positions[i] = pos;
+}
+
+__global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand) {
+  __shared__ long red[16];
+  __shared__ long base_s[1024];
+  __shared__ int back_s[1024];
+  const int T = blockDim.x, tid = threadIdx.x;
+  const int page = 1 << a.lp;
+  const long room = (long)a.width << a.lp;
+  long top = min(max(*a.count, 0), a.pool);
+  // pages of ended requests go back on the stack, in the requests' order
+  for (int b0 = 0; b0 < a.B; b0 += T) {
+    const int b = b0 + tid;
+    long back = 0;
+    if (b < a.B && a.add[b] < 0) back = min(((long)max(a.past[b], 0) + page - 1) >> a.lp, (long)a.width);
+    if (!__syncthreads_or(back > 0)) continue;
+    long total;
+    const long upto = block_scan_incl(back, red, total);
+    base_s[tid] = top + upto - back;
+    back_s[tid] = (int)back;
+    __syncthreads();
+    const int n = min(T, a.B - b0);
+    for (int r = tid >> 6; r < n; r += T >> 6)
+      for (int j = tid & 63; j < back_s[r]; j += 64)
+        if (base_s[r] + j < a.pool) a.free_ids[base_s[r] + j] = a.table[(long)(b0 + r) * a.table_row + j];
+    top = min(top + total, (long)a.pool);
+    __syncthreads();
+  }
+  long tok0 = 0, page0 = 0, out0 = 0, used = 0;
+  for (int b0 = 0; b0 < a.B; b0 += T) {
+    const int b = b0 + tid;
+    const bool in = b < a.B;
+    const long past = in ? a.past[b] : 0, add = in ? a.add[b] : -1;
+    const bool live = add >= 0;
+    bool fits = live && past >= 0 && past + add <= room;
+    long total;
+    const long tok = tok0 + block_scan_incl(fits ? add : 0, red, total);
+    tok0 += total;
+    fits = fits && tok <= a.tokens;
+    const long have = (max(past, 0l) + page - 1) >> a.lp;
+    const long need = fits ? ((past + add + page - 1) >> a.lp) - have : 0;
+    const long upto = page0 + block_scan_incl(need, red, total);
+    page0 += total;
+    const bool granted = fits && (need == 0 || upto <= top);
+    const long out = out0 + block_scan_incl(granted ? add : 0, red, total);
+    out0 += total;
+    block_scan_incl(granted ? need : 0, red, total);
+    used += total;
+    if (in) {
+      a.lens[b] = live ? (int)(past + (granted ? add : 0)) : 0;
+      a.starts[b] = (int)(out - (granted ? add : 0));
+      a.waits[b] = live && !granted ? 1 : 0;
+      a.ws[b] = (int)(upto - need);
+    }
+  }
+  if (tid == 0) {
+    a.starts[a.B] = (int)out0;
+    a.ws[a.B] = (int)top;
+    *a.count_out = (int)(top - used);
+  }
+  if (!expand) return;
+  __syncthreads();
+  for (int i = tid; i < a.tokens; i += T) plan_token(a, i, (int)out0, a.starts, a.ws, (int)top);
+}
+
+__global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < a.tokens) plan_token(a, i, a.starts[a.B], a.starts, a.ws, a.ws[a.B]);
+}
+
+// ---- cache writer -------------------------------------------------------------------------
+// 16 bytes a thread: token, head and vector of a unit; slots outside the cache are skipped.
+__global__ __launch_bounds__(256) void paged_write_kernel(imgcap_paged_write_desc d, int vecs, int lp, int esz) {
+  const unsigned per = (unsigned)d.heads * vecs;
+  const unsigned u = blockIdx.x * 256u + threadIdx.x;
+  if (u >= per * (unsigned)d.n) return;
+  const unsigned tok = u / per, rest = u - tok * per, head = rest / vecs, vec = rest - head * vecs;
+  const long slot = d.slots[tok];
+  if (slot < 0 || (slot >> lp) >= d.pages) return;
+  const long pg = slot >> lp, off = slot & (d.page - 1);
+  const bool second = blockIdx.y != 0;
+  const char* src = (const char*)(second ? d.v : d.k);
+  char* dst = (char*)(second ? d.vc : d.kc);
+  src += ((long)tok * (second ? d.v_row : d.k_row) + (long)head * (second ? d.v_head : d.k_head)) * esz + vec * 16;
+  dst += (pg * (second ? d.vc_page : d.kc_page) + off * (second ? d.vc_tok : d.kc_tok) +
+          (long)head * (second ? d.vc_head : d.kc_head)) * esz + vec * 16;
+  *(uint4*)dst = *(const uint4*)src;
+}
+
+// ---- attention of one new token per request --------------------------------------------------
+// Row = (request, kv head, 16 of the query heads that share it).  A wave takes 32 tokens a step:
+//   S^T[token][head] = K Q^T   (A = 16 tokens of K, B = the queries; the accumulator's column is a
+//                               head, its rows 4 tokens per lane group)
+//   O^T[dh][head]  += V^T P^T  (B = those very registers: lane group g holds tokens 4g..4g+3 of each
+//                               16, so the product's k order is taken to be that, and V's rows are
+//                               read in it: no exchange between lanes, nothing through LDS)
+// with a running maximum and sum per head (base 2).  A lane of V holds DH / 16 consecutive columns
+// of its 4 + 4 tokens; the transposed operand is byte permutes of those words.  fp32 does the same
+// on the exact fp32 instruction, whose k is one token per lane group.
+// Positions past the length, or on a page outside the cache, are not there: score -inf, V zeroed.
+template <int BYTES> struct Words { uint32_t w[BYTES / 4]; };
+template <int BYTES> DEV Words<BYTES> load_words(const void* p) {
+  Words<BYTES> r;
+  if constexpr (BYTES == 8) {
+    const uint2 u = *(const uint2*)p;
+    r.w[0] = u.x; r.w[1] = u.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 u = ((const uint4*)p)[i];
+      r.w[4 * i] = u.x; r.w[4 * i + 1] = u.y; r.w[4 * i + 2] = u.z; r.w[4 * i + 3] = u.w;
+    }
+  }
+  return r;
+}
+
+template <typename T, int DH> struct KvTile {  // 32 tokens of one kv head, as the wave's operands
+  static constexpr int NS = DH * sizeof(T) / 64;   // 16-byte pieces of a key row per lane
+  static constexpr int VB = DH / 16 * sizeof(T);   // bytes of a value row per lane
+  uint4 k[2][NS];
+  Words<VB> v[2][4];
+  bool live[2];  // the page is one of the cache's (pages of 16 tokens and more)
+};
+
+template <typename T, int DH>
+DEV void kv_load(KvTile<T, DH>& t, const imgcap_paged_attn_desc& d, const int32_t* table, int kvh, int tok, int n, int lp) {
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const T* kb = (const T*)d.k + (long)kvh * d.k_head;
+  const T* vb = (const T*)d.v + (long)kvh * d.v_head;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int t0 = tok + 16 * h;
+    if (lp >= 4) {  // the 16 tokens share a page
+      const int id = table[min(t0, n - 1) >> lp];
+      t.live[h] = (unsigned)id < (unsigned)d.pages;
+      const long pg = t.live[h] ? id : 0, off = t0 & (d.page - 1);
+      const T* kp = kb + pg * d.k_page + (off + r) * d.k_tok + g * (16 / sizeof(T));
+      const T* vp = vb + pg * d.v_page + (off + 4 * g) * d.v_tok + r * (DH / 16);
+#pragma unroll
+      for (int s = 0; s < KvTile<T, DH>::NS; ++s) t.k[h][s] = *(const uint4*)(kp + s * (64 / sizeof(T)));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) t.v[h][i] = load_words<KvTile<T, DH>::VB>(vp + i * d.v_tok);
+    } else {
+      const int tk = min(t0 + r, n - 1);
+      const int id = table[tk >> lp];
+      const int slot_page = (unsigned)id < (unsigned)d.pages ? id : -1;
+      const T* kp = kb + (long)max(slot_page, 0) * d.k_page + (tk & (d.page - 1)) * d.k_tok + g * (16 / sizeof(T));
+#pragma unroll
+      for (int s = 0; s < KvTile<T, DH>::NS; ++s) t.k[h][s] = *(const uint4*)(kp + s * (64 / sizeof(T)));
+      t.live[h] = slot_page >= 0;  // of this lane's own token r
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int vi = __shfl(slot_page, 4 * g + i, 64), vt = min(t0 + 4 * g + i, n - 1);
+        const T* vp = vb + (long)max(vi, 0) * d.v_page + (vt & (d.page - 1)) * d.v_tok + r * (DH / 16);
+        t.v[h][i] = load_words<KvTile<T, DH>::VB>(vp);
+      }
+    }
+  }
+}
+
+DEV uint32_t pack_bf16(float a, float b) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (bf16)b) << 16);
+}
+
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit, int gtiles,
+                                                         int lp, float* ws_o, float* ws_ml) {
+  using Tile = KvTile<T, DH>;
+  constexpr int VPL = DH / 16, LDO = DH + 4;
+  extern __shared__ float sm[];  // [waves][16][LDO] of O, then [waves][16] maxima and sums
+  const int nw = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int r = lane & 15, g = lane >> 4;
+  const int row = blockIdx.x, gt = row % gtiles, kvh = (row / gtiles) % d.Hkv, b = row / gtiles / d.Hkv;
+  const int split = blockIdx.y, G = d.H / d.Hkv, heads = min(16, G - 16 * gt), h0 = kvh * G + 16 * gt;
+  const int n = min(max(d.lens[b], 0), d.max_len);
+  if (split > 0 && split * (long)chunk >= n) return;
+  const int t0 = split * chunk, t1 = min(n, t0 + chunk);
+  const int32_t* table = d.table + (long)b * d.table_row;
+  const float c = d.scale * 1.44269504088896341f;
+  uint4 q[Tile::NS];
+#pragma unroll
+  for (int s = 0; s < Tile::NS; ++s) {
+    q[s] = make_uint4(0u, 0u, 0u, 0u);
+    if (r < heads)
+      q[s] = *(const uint4*)((const T*)d.q + (long)b * d.q_row + (long)(h0 + r) * d.q_head + s * (64 / sizeof(T)) +
+                             g * (16 / sizeof(T)));
+  }
+  f32x4 acc[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, l = 0.f;
+  for (int tok = t0 + 32 * w; tok < t1; tok += 32 * nw) {
+    Tile t;
+    kv_load<T, DH>(t, d, table, kvh, tok, n, lp);
+    float p[2][4];
+    float mx = -INFINITY;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      f32x4 s4 = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < Tile::NS; ++s) {
+        if constexpr (sizeof(T) == 2) {
+          s4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[h][s]),
+                                                       __builtin_bit_cast(bf16x8, q[s]), s4, 0, 0, 0);
+        } else {
+          const f32x4 kk = __builtin_bit_cast(f32x4, t.k[h][s]), qq = __builtin_bit_cast(f32x4, q[s]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qq[e], s4, 0, 0, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const bool here = lp >= 4 ? t.live[h] : __shfl((int)t.live[h], 4 * g + i, 64);
+        const bool ok = here && tok + 16 * h + 4 * g + i < t1;
+        p[h][i] = ok ? s4[i] * c : -INFINITY;
+        mx = fmaxf(mx, p[h][i]);
+        if (!ok) {
+#pragma unroll
+          for (int e = 0; e < Tile::VB / 4; ++e) t.v[h][i].w[e] = 0u;
+        }
+      }
+    }
+    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
+    const float alpha = __builtin_amdgcn_exp2f(m - ms);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        p[h][i] = __builtin_amdgcn_exp2f(p[h][i] - ms);
+        l += p[h][i];
+      }
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) acc[j] *= alpha;
+    if constexpr (sizeof(T) == 2) {
+      // the weights go in as their top bf16 bits and the remainder in bf16: 15 bits and more of them,
+      // so the output carries little but its own rounding.  Both pieces are kept positive (the
+      // remainder at least 1e-30, nothing beside a weight that counts): an infinite value times a
+      // zero or negative remainder would turn the infinity into NaN.
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float a = p[e >> 1][2 * (e & 1)], bb = p[e >> 1][2 * (e & 1) + 1];
+        hi[e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, bb), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+        lo[e] = pack_bf16(fmaxf(a - __builtin_bit_cast(float, hi[e] << 16), 1e-30f),
+                          fmaxf(bb - __builtin_bit_cast(float, hi[e] & 0xffff0000u), 1e-30f));
+      }
+      const bf16x8 ph = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+      const bf16x8 pl = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+        uint32_t x[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[e] = __builtin_amdgcn_perm(t.v[e >> 1][2 * (e & 1) + 1].w[j >> 1], t.v[e >> 1][2 * (e & 1)].w[j >> 1], sel);
+        const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph, acc[j], 0, 0, 0);
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl, acc[j], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < VPL; ++j)
+            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[h][i].w[j]), p[h][i], acc[j], 0,
+                                                          0, 0);
+    }
+  }
+  l += __shfl_xor(l, 16, 64);
+  l += __shfl_xor(l, 32, 64);
+  // the waves' parts, joined in LDS: lane (r, g) holds head r, columns VPL * (4g + i) + j
+  float* so = sm + (w * 16 + r) * LDO;
+  float* sml = sm + nw * 16 * LDO;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) so[VPL * (4 * g + i) + j] = acc[j][i];
+  if (g == 0) {
+    sml[w * 16 + r] = m;
+    sml[(nw + w) * 16 + r] = l;
+  }
+  __syncthreads();
+  const bool whole = n <= chunk;
+  for (int e = threadIdx.x; e < heads * DH; e += blockDim.x) {
+    const int hd = e / DH, col = e % DH;
+    float M = -INFINITY;
+    for (int i = 0; i < nw; ++i) M = fmaxf(M, sml[i * 16 + hd]);
+    const float ms = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o = 0.f;
+    for (int i = 0; i < nw; ++i) {
+      const float f = __builtin_amdgcn_exp2f(sml[i * 16 + hd] - ms);
+      L += f * sml[(nw + i) * 16 + hd];
+      o += f * sm[(i * 16 + hd) * LDO + col];
+    }
+    const long bh = (long)b * d.H + h0 + hd;
+    if (whole) {
+      ((T*)d.o)[(long)b * d.o_row + (long)(h0 + hd) * d.o_head + col] = from_f<T>(L == 0.f ? 0.f : o / L);
+      if (d.lse && col == 0) d.lse[bh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+    } else {
+      ws_o[(bh * nsplit + split) * DH + col] = o;
+      if (col == 0) {
+        ws_ml[(bh * nsplit + split) * 2] = M;
+        ws_ml[(bh * nsplit + split) * 2 + 1] = L;
+      }
+    }
+  }
+}
+
+// joins the chunks of a row: out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit,
+                                                         const float* __restrict__ ws_o, const float* __restrict__ ws_ml) {
+  constexpr int C4 = DH / 4, PARTS = 256 / C4;
+  __shared__ float red[4];
+  __shared__ float part[PARTS][DH + 1];
+  const int b = blockIdx.x / d.H, h = blockIdx.x % d.H;
+  const int n = min(max(d.lens[b], 0), d.max_len);
+  if (n <= chunk) return;
+  const int ns = (n + chunk - 1) / chunk;
+  const float* ml = ws_ml + (long)blockIdx.x * nsplit * 2;
+  const float* oo = ws_o + (long)blockIdx.x * nsplit * DH;
+  float M = -INFINITY;
+  for (int s = threadIdx.x; s < ns; s += 256) M = fmaxf(M, ml[2 * s]);
+  M = wave_max(M);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+  __syncthreads();
+  M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float ms = M == -INFINITY ? 0.f : M;
+  const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+  float L = 0.f;
+  for (int s = pt; s < ns; s += PARTS) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s] - ms);
+    L += f * ml[2 * s + 1];
+    o += f * *(const f32x4*)(oo + (long)s * DH + 4 * c4);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[pt][4 * c4 + i] = o[i];
+  if (c4 == 0) part[pt][DH] = L;
+  __syncthreads();
+  if (threadIdx.x < DH) {
+    float v = 0.f, S = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      v += part[i][threadIdx.x];
+      S += part[i][DH];
+    }
+    ((T*)d.o)[(long)b * d.o_row + (long)h * d.o_head + threadIdx.x] = from_f<T>(S == 0.f ? 0.f : v / S);
+    if (d.lse && threadIdx.x == 0) d.lse[blockIdx.x] = S == 0.f ? -INFINITY : (M + log2f(S)) * 0.69314718055994531f;
+  }
+}
+
+static int log2_of(int v) { return __builtin_ctz((unsigned)v); }
+static bool is_pow2(int v) { return v > 0 && (v & (v - 1)) == 0; }
+
+static int attn_check(const imgcap_paged_attn_desc* d) {
+  IMGCAP_REQUIRE(d != nullptr, "paged attention: desc NULL");
+  IMGCAP_REQUIRE(d->dtype == IMGCAP_F32 || d->dtype == IMGCAP_BF16, "paged attention: dtype must be fp32 or bf16");
+  IMGCAP_REQUIRE(d->dh == 64 || d->dh == 128, "paged attention: head dim must be 64 or 128");
+  IMGCAP_REQUIRE(d->B >= 0 && d->Hkv > 0 && d->H > 0 && d->H % d->Hkv == 0,
+                 "paged attention: query heads must be a multiple of the key/value heads");
+  IMGCAP_REQUIRE(is_pow2(d->page) && d->page <= 1024, "paged attention: page must be a power of two, at most 1024");
+  IMGCAP_REQUIRE(d->pages > 0 && d->width > 0 && d->max_len > 0, "paged attention: empty cache, table or max_len");
+  IMGCAP_REQUIRE((int64_t)d->width * d->page < (1ll << 31) && d->max_len <= (int64_t)d->width * d->page,
+                 "paged attention: max_len must be within the table's width, and that below 2^31 tokens");
+  IMGCAP_REQUIRE(d->q && d->k && d->v && d->o && d->table && d->lens, "paged attention: NULL operand");
+  const int64_t vec = d->dtype == IMGCAP_F32 ? 4 : 8;
+  IMGCAP_REQUIRE(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && d->q_row % vec == 0 && d->q_head % vec == 0 &&
+                     d->k_page % vec == 0 && d->k_tok % vec == 0 && d->k_head % vec == 0 && d->v_page % vec == 0 &&
+                     d->v_tok % vec == 0 && d->v_head % vec == 0,
+                 "paged attention: q, k and v must be 16-byte aligned with strides of whole 16 bytes");
+  return 0;
+}
+
+// How the length is cut: workgroups of up to 4 waves, each wave 32 tokens a step
+struct AttnPlan { int gtiles, waves, chunk, nsplit; };
+static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
+  AttnPlan p;
+  p.gtiles = (d->H / d->Hkv + 15) / 16;
+  p.waves = d->max_len <= 32 ? 1 : d->max_len <= 64 ? 2 : 4;
+  const int64_t rows = (int64_t)d->B * d->Hkv * p.gtiles;
+  const int64_t most = (d->max_len + 255) / 256;
+  int64_t want = rows > 0 ? (1024 + rows - 1) / rows : 1;
+  if (want > most) want = most;
+  if (want < 1) want = 1;
+  p.chunk = (int)(((d->max_len + want - 1) / want + 127) / 128 * 128);
+  p.nsplit = (d->max_len + p.chunk - 1) / p.chunk;
+  return p;
+}
+static int64_t attn_ws(const imgcap_paged_attn_desc* d, const AttnPlan& p) {
+  return p.nsplit > 1 ? (int64_t)d->B * d->H * p.nsplit * (d->dh + 2) * 4 : 0;
+}
+
+template <typename T, int DH>
+static void attn_launch(const imgcap_paged_attn_desc* d, const AttnPlan& p, hipStream_t st) {
+  float* ws_o = (float*)d->ws;
+  float* ws_ml = ws_o ? ws_o + (int64_t)d->B * d->H * p.nsplit * DH : nullptr;
+  const int lds = (p.waves * 16 * (DH + 4) + 2 * p.waves * 16) * 4;
+  hipLaunchKernelGGL((paged_attn_kernel<T, DH>), dim3(d->B * d->Hkv * p.gtiles, p.nsplit), dim3(64 * p.waves), lds, st,
+                     *d, p.chunk, p.nsplit, p.gtiles, log2_of(d->page), ws_o, ws_ml);
+  if (p.nsplit > 1)
+    hipLaunchKernelGGL((paged_join_kernel<T, DH>), dim3(d->B * d->H), dim3(256), 0, st, *d, p.chunk, p.nsplit, ws_o,
+                       ws_ml);
+}
+
+}  // namespace imgcap
+
+using namespace imgcap;
+
+extern "C" int imgcap_paged_plan(int B, int width, int page, int pool, int tokens, const int32_t* past,
+                                 const int32_t* add, int32_t* table, int64_t table_row, int32_t* free_ids,
+                                 const int32_t* count, int32_t* count_out, int32_t* lens, int32_t* starts,
+                                 int64_t* slots, int32_t* rows, int64_t* positions, int32_t* waits, int32_t* ws,
+                                 void* stream) {
+  IMGCAP_REQUIRE(B > 0 && width > 0 && pool > 0 && tokens >= 0, "imgcap_paged_plan: B, width and pool must be positive");
+  IMGCAP_REQUIRE(is_pow2(page) && page <= 1024, "imgcap_paged_plan: page must be a power of two, at most 1024");
+  IMGCAP_REQUIRE((int64_t)width * page < (1ll << 31), "imgcap_paged_plan: width * page must be below 2^31");
+  IMGCAP_REQUIRE(table_row >= width, "imgcap_paged_plan: table rows overlap");
+  IMGCAP_REQUIRE(past && add && table && free_ids && count && count_out && lens && starts && waits && ws &&
+                     (tokens == 0 || (slots && rows && positions)),
+                 "imgcap_paged_plan: NULL operand");
+  const PlanArgs a{B, width, log2_of(page), pool, tokens, past, add, table, (long)table_row, free_ids, count, count_out,
+                   lens, starts, slots, rows, positions, waits, ws};
+  const int threads = B >= 1024 || tokens >= 1024 ? 1024 : ((B > tokens ? B : tokens) + 63) / 64 * 64;
+  const bool one = tokens <= 4096;
+  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(threads), 0, (hipStream_t)stream, a, one ? 1 : 0);
+  if (!one)
+    hipLaunchKernelGGL(paged_slots_kernel, dim3((tokens + 255) / 256), dim3(256), 0, (hipStream_t)stream, a);
+  IMGCAP_CHECK_LAUNCH("imgcap_paged_plan");
+  return 0;
+}
+
+extern "C" int imgcap_paged_write(const imgcap_paged_write_desc* d, void* stream) {
+  IMGCAP_REQUIRE(d != nullptr, "imgcap_paged_write: desc NULL");
+  IMGCAP_REQUIRE(d->dtype == IMGCAP_F32 || d->dtype == IMGCAP_BF16, "imgcap_paged_write: dtype must be fp32 or bf16");
+  const int esz = d->dtype == IMGCAP_F32 ? 4 : 2, vec = 16 / esz;
+  IMGCAP_REQUIRE(d->n >= 0 && d->heads > 0 && d->dh > 0 && d->dh % vec == 0,
+                 "imgcap_paged_write: head dim must be whole 16-byte pieces");
+  IMGCAP_REQUIRE(is_pow2(d->page) && d->page <= 1024 && d->pages > 0,
+                 "imgcap_paged_write: page must be a power of two, at most 1024");
+  if (d->n == 0) return 0;
+  IMGCAP_REQUIRE(d->k && d->v && d->kc && d->vc && d->slots, "imgcap_paged_write: NULL operand");
+  const int64_t st[] = {d->k_row, d->k_head, d->v_row, d->v_head, d->kc_page, d->kc_tok, d->kc_head, d->vc_page,
+                        d->vc_tok, d->vc_head};
+  for (int64_t s : st) IMGCAP_REQUIRE(s % vec == 0, "imgcap_paged_write: strides must be whole 16-byte pieces");
+  IMGCAP_REQUIRE(aligned16(d->k) && aligned16(d->v) && aligned16(d->kc) && aligned16(d->vc),
+                 "imgcap_paged_write: operands must be 16-byte aligned");
+  const int vecs = d->dh / vec;
+  const int64_t units = (int64_t)d->n * d->heads * vecs;
+  IMGCAP_REQUIRE(units < (1ll << 31), "imgcap_paged_write: at most 2^31 16-byte pieces a call");
+  hipLaunchKernelGGL(paged_write_kernel, dim3((unsigned)((units + 255) / 256), 2), dim3(256), 0, (hipStream_t)stream,
+                     *d, vecs, log2_of(d->page), esz);
+  IMGCAP_CHECK_LAUNCH("imgcap_paged_write");
+  return 0;
+}
+
+extern "C" int imgcap_paged_attention_ws(const imgcap_paged_attn_desc* d, int64_t* bytes) {
+  if (int rc = attn_check(d)) return rc;
+  IMGCAP_REQUIRE(bytes != nullptr, "imgcap_paged_attention_ws: bytes NULL");
+  *bytes = attn_ws(d, attn_plan(d));
+  return 0;
+}
+
+extern "C" int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream) {
+  if (int rc = attn_check(d)) return rc;
+  if (d->B == 0) return 0;
+  const AttnPlan p = attn_plan(d);
+  IMGCAP_REQUIRE((int64_t)d->B * d->Hkv * p.gtiles < (1ll << 31) && (int64_t)d->B * d->H < (1ll << 31) &&
+                     p.nsplit <= 65535,
+                 "imgcap_paged_attention: too many rows");
+  const int64_t need = attn_ws(d, p);
+  if (need > 0 && !(d->ws && aligned16(d->ws) && d->ws_bytes >= need))
+    return fail(IMGCAP_EWORKSPACE, "imgcap_paged_attention: " + std::to_string(need) +
+                                       " bytes of 16-byte aligned workspace needed (imgcap_paged_attention_ws)");
+  hipStream_t st = (hipStream_t)stream;
+  if (d->dtype == IMGCAP_BF16) {
+    if (d->dh == 64) attn_launch<bf16, 64>(d, p, st);
+    else attn_launch<bf16, 128>(d, p, st);
+  } else {
+    if (d->dh == 64) attn_launch<float, 64>(d, p, st);
+    else attn_launch<float, 128>(d, p, st);
+  }
+  IMGCAP_CHECK_LAUNCH("imgcap_paged_attention");
+  return 0;
+}

@@ -614,6 +614,200 @@ def transpose(x, out=None):
     return out
 
 
+# ---- paged key/value cache and token log-probabilities ------------------------------------------
+def _one_device(name, *ts):
+    """The GPU that all of ``ts`` (None left out) live on."""
+    dev = ts[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _call_on(dev, name, *args):
+    """``name`` on the current stream of ``dev``, whichever device is the current one."""
+    if dev.index == torch.cuda.current_device():
+        _abi.call(name, *args, stream())
+    else:
+        with torch.cuda.device(dev):
+            _abi.call(name, *args, stream())
+
+
+def _want(name, what, t, dtype, shape, contiguous=True):
+    if t.dtype != dtype:
+        raise TypeError(f"{name}: {what} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name}: {what} must have shape {shape}, got {tuple(t.shape)}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"{name}: {what} must be contiguous")
+
+
+def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, out=None):
+    """Pages, slots and positions of one step's new tokens from the requests' lengths, on the GPU
+    (imgcap_paged_plan): request b, with past[b] tokens in the cache, gets new[b] more, or has ended
+    (new[b] < 0: its pages go back).  ``table`` [B, width] int32 gets the new pages' ids, which come
+    from the end of the stack ``free`` [pool] int32 holding ``count`` [1] int32 of them; the number
+    left goes to ``count_out`` (default: count itself).  ``tokens`` is the step's capacity, at least
+    the sum of new.  Returns (lens [B] int32, starts [B + 1] int32, slots [tokens] int64, rows
+    [tokens] int32, positions [tokens] int64, waits [B] int32); pass it back as ``out`` to have it
+    filled again (a captured graph's outputs).  A request that does not fit -- lengths past the table,
+    no page left, no token left -- waits: waits[b] = 1, nothing else of it changes."""
+    count_out = count if count_out is None else count_out
+    dev = _one_device("paged_plan", past, new, table, free, count, count_out)
+    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+        raise ValueError("paged_plan: table must be [B, width] int32 with unit inner stride")
+    B, width = table.shape
+    _want("paged_plan", "past", past, torch.int32, (B,))
+    _want("paged_plan", "new", new, torch.int32, (B,))
+    _want("paged_plan", "free", free, torch.int32, (free.numel(),))
+    _want("paged_plan", "count", count, torch.int32, (1,))
+    _want("paged_plan", "count_out", count_out, torch.int32, (1,))
+    if out is None:
+        i32, i64 = dict(device=dev, dtype=torch.int32), dict(device=dev, dtype=torch.int64)
+        out = (torch.empty(B, **i32), torch.empty(B + 1, **i32), torch.empty(tokens, **i64),
+               torch.empty(tokens, **i32), torch.empty(tokens, **i64), torch.empty(B, **i32))
+    else:
+        _one_device("paged_plan", past, *out)
+        for what, t, dtype, n in zip(("lens", "starts", "slots", "rows", "positions", "waits"), out,
+                                     (torch.int32, torch.int32, torch.int64, torch.int32, torch.int64, torch.int32),
+                                     (B, B + 1, tokens, tokens, tokens, B)):
+            _want("paged_plan", what, t, dtype, (n,))
+    lens, starts, slots, rows, positions, waits = out
+    ws = torch.empty(B + 1, device=dev, dtype=torch.int32)
+    _call_on(dev, "imgcap_paged_plan", B, width, page, free.numel(), tokens, past.data_ptr(), new.data_ptr(),
+             table.data_ptr(), table.stride(0) if B > 1 else width, free.data_ptr(), count.data_ptr(),
+             count_out.data_ptr(), lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), rows.data_ptr(),
+             positions.data_ptr(), waits.data_ptr(), ws.data_ptr())
+    return out
+
+
+def _cache_pair(name, k, v):
+    if k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"{name}: caches must be [pages, page, kv heads, head dim], both alike")
+    if k.stride(3) != 1 or v.stride(3) != 1:
+        raise ValueError(f"{name}: caches must have unit inner stride")
+    return k.shape
+
+
+def paged_write(k, v, k_cache, v_cache, slots):
+    """k_cache[slot // page, slot % page] = k[i] for slot = slots[i] (int64, imgcap_paged_write), and
+    the values alike: k / v [n, kv heads, head dim] views, caches [pages, page, kv heads, head dim] of
+    any strides.  A slot outside the cache (-1: padding) is skipped.  Slots of one call are distinct."""
+    dev = _one_device("paged_write", k, v, k_cache, v_cache, slots)
+    pages, page, heads, dh = _cache_pair("paged_write", k_cache, v_cache)
+    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
+        raise TypeError("paged_write: k, v and the caches must share a dtype")
+    n = slots.numel()
+    _want("paged_write", "slots", slots, torch.int64, (n,))
+    if tuple(k.shape) != (n, heads, dh) or tuple(v.shape) != (n, heads, dh):
+        raise ValueError(f"paged_write: k and v must be [{n}, {heads}, {dh}]")
+    if n and (k.stride(2) != 1 or v.stride(2) != 1):
+        raise ValueError("paged_write: k and v must have unit inner stride")
+    d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                            *k_cache.stride()[:3], *v_cache.stride()[:3], k.data_ptr(), v.data_ptr(),
+                            k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr())
+    _call_on(dev, "imgcap_paged_write", ctypes.byref(d))
+
+
+def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=None, out=None, lse=None):
+    """Attention of one new token per request over its pages (imgcap_paged_attention): q [B, H, head
+    dim], caches [pages, page, kv heads, head dim] of any strides, table [B, width] int32, lens [B]
+    int32 -> out [B, H, head dim].  H is a multiple of the kv heads, head dim 64 or 128, fp32 or bf16.
+    ``max_len`` (default: the table's width) bounds the lengths from the host; the work is cut for it.
+    A request of length 0 gets zeros; positions on a page outside the cache are not there.
+    ``lse`` [B, H] fp32 gets the natural log-sum-exp of the scores (default scale: head dim ** -0.5)."""
+    dev = _one_device("paged_attention", q, k_cache, v_cache, table, lens, out, lse)
+    pages, page, hkv, dh = _cache_pair("paged_attention", k_cache, v_cache)
+    if q.dim() != 3 or q.shape[2] != dh:
+        raise ValueError(f"paged_attention: q must be [B, H, {dh}]")
+    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+        raise TypeError("paged_attention: q and the caches must share a dtype")
+    B, H = q.shape[:2]
+    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B or table.stride(1) != 1:
+        raise ValueError("paged_attention: table must be [B, width] int32 with unit inner stride")
+    _want("paged_attention", "lens", lens, torch.int32, (B,))
+    if out is None:
+        out = torch.empty(B, H, dh, device=dev, dtype=q.dtype)
+    else:
+        _want("paged_attention", "out", out, q.dtype, (B, H, dh), contiguous=False)
+    if q.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("paged_attention: q and out must have unit inner stride")
+    if lse is not None:
+        _want("paged_attention", "lse", lse, torch.float32, (B, H))
+    if B == 0:
+        return out
+    width = table.shape[1]
+    d = _abi.PagedAttnDesc(dt(q), B, H, hkv, dh, page, pages, width, width * page if max_len is None else max_len,
+                           dh ** -0.5 if scale is None else scale, q.stride(0), q.stride(1), out.stride(0),
+                           out.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0), q.data_ptr(),
+                           k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), ptr(lse), table.data_ptr(),
+                           lens.data_ptr(), None, 0)
+    need = ctypes.c_int64(0)
+    _abi.check("imgcap_paged_attention_ws", ctypes.byref(d), ctypes.byref(need))
+    if need.value:  # a split length: the parts' maxima, sums and outputs
+        ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+        d.ws, d.ws_bytes = ws.data_ptr(), need.value
+    _call_on(dev, "imgcap_paged_attention", ctypes.byref(d))
+    return out
+
+
+def token_logprobs(logits, targets=None, V=None, *, top=0):
+    """Log-probability of ``targets`` [n] int64, entropy and the ``top`` best alternatives of the
+    logit rows ``logits`` [n, >= V] (columns from V on are padding), in one call
+    (imgcap_token_logprobs) -> (logp [n] fp32 or None without targets, entropy [n] fp32 in nats, stats
+    [n, 2] fp32 for token_logprobs_bwd, top_logp [n, top] fp32, top_ids [n, top] int64).  A target
+    outside [0, V) (-1: padding) gives logp 0.  Alternatives come in falling order, equal ones by
+    index, NaN last.  Logits of -inf have no weight; a row of them alone gives -inf and entropy 0."""
+    dev = _one_device("token_logprobs", logits, targets)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("token_logprobs: logits must be [n, V] with unit inner stride")
+    n = logits.shape[0]
+    V = logits.shape[1] if V is None else V
+    if not 0 < V <= logits.shape[1]:
+        raise ValueError(f"token_logprobs: V must be in 1 .. {logits.shape[1]}")
+    if targets is not None:
+        _want("token_logprobs", "targets", targets, torch.int64, (n,))
+    f32 = dict(device=dev, dtype=torch.float32)
+    logp = None if targets is None else torch.empty(n, **f32)
+    entropy, stats, top_logp = torch.empty(n, **f32), torch.empty(n, 2, **f32), torch.empty(n, top, **f32)
+    top_ids = torch.empty(n, top, device=dev, dtype=torch.int64)
+    _call_on(dev, "imgcap_token_logprobs", dt(logits), n, V, top, logits.data_ptr(), logits.stride(0), ptr(targets),
+             ptr(logp), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+    return logp, entropy, stats, top_logp, top_ids
+
+
+def token_logprobs_bwd(logits, targets, stats, entropy, dlogp=None, dentropy=None, *, V=None, dlogits=None):
+    """Gradient of the logits of token_logprobs from those of logp and entropy ([n] fp32, either may
+    be None) -> dlogits [n, V] in the logits' dtype (of a given ``dlogits`` [n, >= V], which may be
+    ``logits`` itself, the columns from V on stay).  The alternatives have no gradient."""
+    dev = _one_device("token_logprobs_bwd", logits, targets, stats, entropy, dlogp, dentropy, dlogits)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError("token_logprobs_bwd: logits must be [n, V] with unit inner stride")
+    n = logits.shape[0]
+    V = logits.shape[1] if V is None else V
+    if not 0 < V <= logits.shape[1]:
+        raise ValueError(f"token_logprobs_bwd: V must be in 1 .. {logits.shape[1]}")
+    if dlogp is not None and targets is None:
+        raise ValueError("token_logprobs_bwd: dlogp needs the targets")
+    if targets is not None:
+        _want("token_logprobs_bwd", "targets", targets, torch.int64, (n,))
+    _want("token_logprobs_bwd", "stats", stats, torch.float32, (n, 2))
+    for what, t in (("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
+        if t is not None:
+            _want("token_logprobs_bwd", what, t, torch.float32, (n,))
+    if dlogits is None:
+        vec = 16 // logits.element_size()  # rows on whole 16-byte vectors
+        dlogits = torch.empty(n, (V + vec - 1) // vec * vec, device=dev, dtype=logits.dtype)[:, :V]
+    elif dlogits.dtype != logits.dtype or dlogits.dim() != 2 or dlogits.shape[0] != n or dlogits.shape[1] < V \
+            or dlogits.stride(1) != 1:
+        raise ValueError("token_logprobs_bwd: dlogits must be [n, >= V] in the logits' dtype with unit inner stride")
+    _call_on(dev, "imgcap_token_logprobs_bwd", dt(logits), n, V, logits.data_ptr(), logits.stride(0), ptr(targets),
+             stats.data_ptr(), entropy.data_ptr(), ptr(dlogp), ptr(dentropy), dlogits.data_ptr(), dlogits.stride(0))
+    return dlogits
+
+
 _seed_counter = None  # the registered counter tensor, kept alive while the library points at it
 
 

@@ -53,8 +53,9 @@ int imgcap_workspace_attach(int slot, void* ptr, uint64_t bytes);
 int imgcap_workspace_needed(int slot, uint64_t* bytes);
 /* ABI revision of this header; imgcap_version() returns the library's.  Bumped whenever an
  * entry point changes meaning or arity (6: imgcap_add_layernorm_bwd's per-block partials
- * argument, imgcap_gemm_get_pt; bindings refuse a library of another revision). */
-#define IMGCAP_ABI_VERSION 6
+ * argument, imgcap_gemm_get_pt; 7: the paged cache and token log-probability entry points;
+ * bindings refuse a library of another revision). */
+#define IMGCAP_ABI_VERSION 7
 int imgcap_version(void);
 
 /* Device-resident step counter mixed into every dropout / stochastic-depth seed at kernel
@@ -504,6 +505,87 @@ int imgcap_mean_mid(int dtype, int B, int P, int E, const void* x, void* out, vo
 int imgcap_sort_gather_rows(int dtype, int B, int P, int E, int L, const int64_t* lens, const void* enc,
                             const int64_t* caps, void* enc_out, void* mean_out, int64_t* caps_out, int64_t* sort_ind,
                             int32_t* dl, void* stream);
+
+/* ---------------------------------------------------------------------------------------
+ * Paged key/value cache of incremental decoding.  A cache is [pages][page][kv heads][dh]; the
+ * page size is a power of two up to 1024; request b owns the pages table[b, 0 .. ceil(len/page)),
+ * and its position p sits in slot table[b, p / page] * page + p % page.
+ *
+ * imgcap_paged_plan: one step's pages, slots and positions from the requests' lengths.
+ *   past[B]   tokens of request b in the cache; add[B] tokens it gets now, negative: it has ended
+ *   table     [B, table_row] int32; entries of the pages a request holds are read, those of the
+ *             pages it gets are written (nothing else of it is)
+ *   free_ids  [pool] int32: the free pages are free_ids[0 .. *count); ended requests' pages are
+ *             pushed on its end first, in the requests' order, then pages are taken from its end
+ *   count_out the free pages left (may be count itself)
+ * A request gets its tokens if past >= 0, past + add <= width * page, the tokens asked up to and
+ * with it stay within `tokens`, and the new pages asked up to and with it are there (one that needs
+ * no page does not wait for others).  Otherwise waits[b] = 1 and it stays as it is.
+ *   lens[B] = past + granted tokens (0: ended), starts[B + 1] = prefix sums of the granted tokens;
+ *   token i of the step: slots[i], rows[i] its request, positions[i]; behind the last one -1, -1, 0,
+ *   and slot -1 where the page's id is outside [0, pool).
+ *   ws: B + 1 int32 of scratch.  Requests must not share the pages that one of them gives back. */
+int imgcap_paged_plan(int B, int width, int page, int pool, int tokens, const int32_t* past, const int32_t* add,
+                      int32_t* table, int64_t table_row, int32_t* free_ids, const int32_t* count,
+                      int32_t* count_out, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* rows,
+                      int64_t* positions, int32_t* waits, int32_t* ws, void* stream);
+
+/* Key and value rows k/v [n, heads, dh] (element strides *_row, *_head; unit inner stride) to their
+ * slots of the two caches (element strides *_page, *_tok, *_head).  A slot outside [0, pages * page)
+ * is skipped.  16-byte aligned operands, all strides whole 16-byte pieces.  The slots of one call are
+ * distinct (of two rows with one slot, either's pieces may stand). */
+typedef struct imgcap_paged_write_desc {
+  int32_t dtype, n, heads, dh, page, pages;
+  int64_t k_row, k_head, v_row, v_head;
+  int64_t kc_page, kc_tok, kc_head, vc_page, vc_tok, vc_head;
+  const void* k;
+  const void* v;
+  void* kc;
+  void* vc;
+  const int64_t* slots;
+} imgcap_paged_write_desc;
+int imgcap_paged_write(const imgcap_paged_write_desc* d, void* stream);
+
+/* Attention of one new token per request over its pages: o[b, h] = softmax(scale q[b, h] . k) v over
+ * the positions [0, min(lens[b], max_len)) of request b; query heads h * Hkv / H share a kv head.
+ * dh 64 or 128.  Positions on a page whose id is outside [0, pages) are not there.  A request without
+ * a position (or whose every score is -inf) gets 0 and lse -inf.  lse (optional): natural log-sum-exp
+ * of the scaled scores, [B, H] contiguous.  q, k, v 16-byte aligned with strides of whole 16 bytes.
+ * max_len bounds the lengths on the host side: the launch is cut for it, and longer rows end there.
+ * ws: imgcap_paged_attention_ws bytes, 16-byte aligned, the call's own until it has run. */
+typedef struct imgcap_paged_attn_desc {
+  int32_t dtype, B, H, Hkv, dh, page, pages, width, max_len;
+  float scale;
+  int64_t q_row, q_head, o_row, o_head;
+  int64_t k_page, k_tok, k_head, v_page, v_tok, v_head;
+  int64_t table_row;
+  const void* q;
+  const void* k;
+  const void* v;
+  void* o;
+  float* lse;
+  const int32_t* table;
+  const int32_t* lens;
+  void* ws;
+  int64_t ws_bytes;
+} imgcap_paged_attn_desc;
+int imgcap_paged_attention_ws(const imgcap_paged_attn_desc* d, int64_t* bytes);
+int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream);
+
+/* Log-probability of given tokens, entropy and the `top` (0 .. min(64, V)) best alternatives of
+ * logit rows [n, V] (pitch ld): logp[n] (0 where the target is outside [0, V); targets may be NULL),
+ * entropy[n] in nats, stats[n, 2] = (maximum, log of the sum of e^(x - maximum)) for the backward,
+ * top_logp / top_ids [n, top] in falling order, ties to the lower index, NaN last.  Logits of -inf
+ * have no weight; a row of them alone gives logp -inf and entropy 0. */
+int imgcap_token_logprobs(int dtype, int n, int V, int top, const void* logits, int64_t ld, const int64_t* targets,
+                          float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids,
+                          void* stream);
+/* Its gradient: dlogits[n, V] (pitch ldd, written; in place of the logits if the pitches agree) from
+ * dlogp[n] and dentropy[n] (either may be NULL = 0); a row whose target is outside [0, V) has none
+ * from dlogp.  The alternatives are not differentiated. */
+int imgcap_token_logprobs_bwd(int dtype, int n, int V, const void* logits, int64_t ld, const int64_t* targets,
+                              const float* stats, const float* entropy, const float* dlogp, const float* dentropy,
+                              void* dlogits, int64_t ldd, void* stream);
 
 /* elementwise helpers */
 int imgcap_cast(int in_dtype, int out_dtype, int64_t n, const void* x, void* y, void* stream);

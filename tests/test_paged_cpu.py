@@ -1,0 +1,126 @@
+"""Refusals of the paged-cache and token log-probability entry points at the C boundary: every call
+here is turned down before anything is launched (there is no GPU), with a message that says why."""
+import ctypes
+
+import pytest
+import torch
+
+from imagecaptioningconvnext_amd import _abi
+from imagecaptioningconvnext_amd import kernels as K
+
+A = 1 << 20  # an aligned address that is never read: the calls are refused on the host
+
+
+def _attn(**kw):
+    d = _abi.PagedAttnDesc(_abi.BF16, 2, 8, 2, 64, 16, 10, 4, 64, 0.125, 512, 64, 512, 64, 2048, 128, 64, 2048, 128, 64,
+                           4, A, A, A, A, None, A, A, None, 0)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _said():
+    return _abi.lib().imgcap_last_error_string().decode()
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(dtype=2), "dtype"), (dict(dh=96), "head dim"), (dict(dh=0), "head dim"), (dict(H=9), "multiple"),
+    (dict(Hkv=0), "multiple"), (dict(H=0), "multiple"), (dict(B=-1), "multiple"), (dict(page=12), "power of two"),
+    (dict(page=0), "power of two"), (dict(page=2048), "power of two"), (dict(pages=0), "empty"), (dict(width=0), "empty"),
+    (dict(max_len=0), "empty"), (dict(max_len=65), "max_len"), (dict(width=1 << 30), "2^31"), (dict(q=None), "NULL"),
+    (dict(k=None), "NULL"), (dict(lens=None), "NULL"), (dict(table=None), "NULL"), (dict(o=None), "NULL"),
+    (dict(q=A + 2), "16-byte"), (dict(v=A + 8), "16-byte"), (dict(k_tok=129), "16"), (dict(v_head=60), "16"),
+    (dict(q_row=511), "16"), (dict(k_page=2047), "16"),
+])
+def test_attention_refuses(kw, why):
+    d, need = _attn(**kw), ctypes.c_int64(-1)
+    assert _abi.lib().imgcap_paged_attention(ctypes.byref(d), None) == -1
+    assert why in _said()
+    assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == -1
+    assert need.value == -1
+
+
+def test_attention_needs_its_workspace():
+    """A split length without the workspace is refused as such, and the size asked for is enough to
+    hold a maximum, a sum and an output per part."""
+    d, need = _attn(width=4096, max_len=65536), ctypes.c_int64(0)
+    assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == 0
+    assert need.value >= 2 * 8 * 2 * (64 + 2) * 4
+    for ws, size in ((None, need.value), (A + 4, need.value), (A, need.value - 1)):
+        d.ws, d.ws_bytes = ws, size
+        assert _abi.lib().imgcap_paged_attention(ctypes.byref(d), None) == _abi.IMGCAP_EWORKSPACE
+    assert _abi.lib().imgcap_paged_attention(None, None) == -1
+    empty = _attn(B=0)
+    assert _abi.lib().imgcap_paged_attention(ctypes.byref(empty), None) == 0
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(dtype=3), "dtype"), (dict(dh=60), "16-byte"), (dict(heads=0), "16-byte"), (dict(n=-1), "16-byte"),
+    (dict(page=24), "power of two"), (dict(pages=0), "power of two"), (dict(k=None), "NULL"), (dict(slots=None), "NULL"),
+    (dict(k_row=4), "strides"), (dict(vc_tok=12), "strides"), (dict(vc=A + 4), "aligned"), (dict(n=1 << 30), "2^31"),
+])
+def test_write_refuses(kw, why):
+    d = _abi.PagedWriteDesc(_abi.BF16, 3, 8, 64, 16, 10, 512, 64, 512, 64, 8192, 512, 64, 8192, 512, 64, A, A, A, A, A)
+    for k, v in kw.items():
+        setattr(d, k, v)
+    assert _abi.lib().imgcap_paged_write(ctypes.byref(d), None) == -1
+    assert why in _said()
+
+
+def test_write_of_nothing_is_nothing():
+    d = _abi.PagedWriteDesc(_abi.F32, 0, 8, 64, 16, 10, *([0] * 10), None, None, None, None, None)
+    assert _abi.lib().imgcap_paged_write(ctypes.byref(d), None) == 0
+
+
+_PLAN = dict(B=2, width=4, page=16, pool=8, tokens=2, past=A, add=A, table=A, table_row=4, free=A, count=A, count_out=A,
+             lens=A, starts=A, slots=A, rows=A, positions=A, waits=A, ws=A)
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(B=0), "positive"), (dict(width=0), "positive"), (dict(pool=0), "positive"), (dict(tokens=-1), "positive"),
+    (dict(page=3), "power of two"), (dict(page=4096), "power of two"), (dict(width=1 << 28, table_row=1 << 28), "2^31"),
+    (dict(table_row=3), "overlap"), (dict(past=None), "NULL"), (dict(ws=None), "NULL"), (dict(slots=None), "NULL"),
+])
+def test_plan_refuses(kw, why):
+    assert _abi.lib().imgcap_paged_plan(*{**_PLAN, **kw}.values(), None) == -1
+    assert why in _said()
+
+
+@pytest.mark.parametrize("args,why", [
+    ((2, 4, 100, 0, A, 100, None, None, A, A, None, None), "dtype"),
+    ((1, 4, 100, 65, A, 100, None, None, A, A, A, A), "top"), ((1, 4, 8, 9, A, 8, None, None, A, A, A, A), "top"),
+    ((1, 4, 100, -1, A, 100, None, None, A, A, A, A), "top"), ((1, 4, 0, 0, A, 100, None, None, A, A, None, None), "bad"),
+    ((1, -1, 9, 0, A, 9, None, None, A, A, None, None), "bad"), ((1, 4, 100, 0, A, 99, None, None, A, A, None, None), "bad"),
+    ((1, 4, 100, 3, A, 100, None, None, A, A, None, A), "NULL"), ((1, 4, 100, 0, A, 100, A, None, A, A, None, None), "NULL"),
+])
+def test_logprobs_refuses(args, why):
+    assert _abi.lib().imgcap_token_logprobs(*args, None) == -1
+    assert why in _said()
+
+
+@pytest.mark.parametrize("args,why", [
+    ((2, 4, 100, A, 100, A, A, A, A, A, A, 100), "dtype"), ((1, 4, 100, A, 100, A, A, A, A, A, A, 99), "bad"),
+    ((1, 4, 100, A, 100, None, A, A, A, A, A, 100), "NULL"), ((1, 4, 100, A, 100, A, None, A, A, A, A, 100), "NULL"),
+    ((1, 4, 100, A, 100, A, A, A, A, A, A, 104), "in place"),
+])
+def test_logprobs_bwd_refuses(args, why):
+    assert _abi.lib().imgcap_token_logprobs_bwd(*args, None) == -1
+    assert why in _said()
+
+
+def test_no_rows_is_nothing():
+    L = _abi.lib()
+    assert L.imgcap_token_logprobs(1, 0, 10, 3, None, 10, None, None, None, None, None, None, None) == 0
+    assert L.imgcap_token_logprobs_bwd(0, 0, 10, None, 10, None, None, None, None, None, None, 10, None) == 0
+
+
+def test_wrappers_refuse_cpu_tensors():
+    x = torch.zeros(2, 8, 64)
+    c = torch.zeros(4, 16, 8, 64)
+    i = torch.zeros(2, dtype=torch.int32)
+    t = torch.zeros(2, 4, dtype=torch.int32)
+    for call in (lambda: K.paged_attention(x, c, c, t, i), lambda: K.paged_write(x, x, c, c, i.long()),
+                 lambda: K.paged_plan(i, i, t, i, i[:1], 16, 2), lambda: K.token_logprobs(x[0]),
+                 lambda: K.token_logprobs_bwd(x[0], None, x[0], x[0, 0])):
+        with pytest.raises(RuntimeError, match="GPU"):
+            call()
