@@ -222,12 +222,16 @@ def _grow_workspaces(dev):
             _attach(dev, slot, need.value * 5 // 4)
 
 
+def fail(name, rc):
+    msg = lib().imgcap_last_error_string().decode(errors="replace")
+    raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+
+
 def check(name, *args):
     """Call an entry point that only computes on the host (no workspace is attached for it)."""
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        msg = lib().imgcap_last_error_string().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+        fail(name, rc)
 
 
 def call(name, *args):
@@ -242,5 +246,4 @@ def call(name, *args):
         _grow_workspaces(dev)
         rc = getattr(lib(), name)(*args)
     if rc != 0:
-        msg = lib().imgcap_last_error_string().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+        fail(name, rc)

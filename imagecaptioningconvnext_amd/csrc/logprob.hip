@@ -36,20 +36,24 @@ template <typename T> struct Row {
   int skew, nvec, V;
   DEV Row(const T* x, int V_) : V(V_) {
     skew = (int)(((uintptr_t)x & 15) / sizeof(T));
-    base = (const uint4*)((uintptr_t)x & ~(uintptr_t)15);
+    base = (const uint4*)((const char*)x - skew * sizeof(T));
     nvec = (V + skew + VEC - 1) / VEC;
   }
-  // vector q with -inf in the places outside the row
-  DEV uint4 load(int q) const {
-    uint4 u = base[q];
+  // -inf in the places of vector q outside the row (the first and the last vector can have such);
+  // on words, so that a row in registers stays one
+  DEV void trim(uint4& u, int q) const {
     const int c0 = q * VEC - skew;
-    if (c0 < 0 || c0 + VEC > V) {
-      T* e = (T*)&u;
+    uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-      for (int i = 0; i < VEC; ++i)
-        if (c0 + i < 0 || c0 + i >= V) e[i] = (T)-INFINITY;
+    for (int i = 0; i < 4; ++i) {
+      if (sizeof(T) == 4) {
+        if (c0 + i < 0 || c0 + i >= V) w[i] = 0xff800000u;
+      } else {
+        if (c0 + 2 * i < 0 || c0 + 2 * i >= V) w[i] = (w[i] & 0xffff0000u) | 0xff80u;
+        if (c0 + 2 * i + 1 < 0 || c0 + 2 * i + 1 >= V) w[i] = (w[i] & 0xffffu) | 0xff800000u;
+      }
     }
-    return u;
+    u = make_uint4(w[0], w[1], w[2], w[3]);
   }
 };
 template <typename T> DEV void unpack(const uint4& u, float (&v)[16 / sizeof(T)]) {
@@ -66,6 +70,13 @@ template <typename T> DEV void unpack(const uint4& u, float (&v)[16 / sizeof(T)]
   }
 }
 
+// The packed words stay what is kept between two passes over a row: without this the compiler keeps
+// the first pass's unpacked floats instead, twice the registers, and spills.
+template <int NV> DEV void keep_packed(uint4 (&u)[NV]) {
+#pragma unroll
+  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(u[j].x), "+v"(u[j].y), "+v"(u[j].z), "+v"(u[j].w));
+}
+
 // (maximum, sum, weighted sum) of two parts of a row; e^(m - M) of a part without weight is not
 // taken, and a difference that passes the float range weighs nothing
 DEV void lp_join(float& m, float& s, float& t, float m2, float s2, float t2) {
@@ -77,18 +88,18 @@ DEV void lp_join(float& m, float& s, float& t, float m2, float s2, float t2) {
   m = M;
 }
 
-// A row per workgroup.  The row is read once into registers (NV vectors a thread; longer rows in
+// A row per workgroup.  The row is read once into registers, NV vectors a thread (a LONG row in
 // segments of that).  Every thread sums relative to its own running maximum, so the row needs one
 // exchange between waves.  Alternatives: the top-th largest of 64 partial maxima (one per lane,
 // over the waves) is a value that at least `top` elements reach; the few elements that reach it are
 // gathered in LDS and ranked there.  Where more than LP_CAND do (long ties), or too few (NaN), the
 // alternatives are found one by one, in passes over the row.
-template <typename T, int TPB, int NV>
-__global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, const T* __restrict__ logits, long ld,
-                                                             const int64_t* __restrict__ tgt, float* __restrict__ logp,
-                                                             float* __restrict__ entropy, float* __restrict__ stats,
-                                                             float* __restrict__ top_logp, int64_t* __restrict__ top_ids) {
-  constexpr int VEC = 16 / sizeof(T), NW = TPB / 64;
+template <typename T, int TPB, int NV, bool LONG>
+__global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void token_logprobs_kernel(
+    int V, int top, const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float* __restrict__ logp,
+    float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logp,
+    int64_t* __restrict__ top_ids) {
+  constexpr int VEC = 16 / sizeof(T), NW = TPB / 64, SEG = TPB * NV;
   __shared__ float part[NW][3];
   __shared__ float lane_max[NW][64];
   __shared__ uint64_t cand[LP_CAND];
@@ -97,44 +108,54 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
   const T* x = logits + row * ld;
   const Row<T> r(x, V);
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
-  const long k = tgt && tid == 0 ? tgt[row] : -1;
+  const long k = tgt ? tgt[row] : -1;
   const bool hit = k >= 0 && k < V;
-  const float xt = hit ? to_f(x[k]) : 0.f;
+  float xt = 0.f;
   if (tid == 0) ncand = 0;
-  const uint4 none4 = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u)
-                                     : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+  constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
   uint4 u[NV];
   float m = -INFINITY, s = 0.f, t = 0.f;
-  for (int q0 = 0; q0 < r.nvec; q0 += TPB * NV) {
+  for (int q0 = 0; q0 < (LONG ? r.nvec : 1); q0 += SEG) {
+    const int last = r.nvec - 1 - q0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      const int q = q0 + j * TPB + tid;
-      u[j] = none4;
-      if (q < r.nvec) u[j] = r.load(q);
-    }
+    for (int j = 0; j < NV; ++j)  // all in flight before the first is used: under no branch, the end again where past it
+      u[j] = r.base[q0 + min(j * TPB + tid, last)];
+    if (q0 == 0 && tid == 0) r.trim(u[0], 0);
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+      if (last >= j * TPB && last < (j + 1) * TPB) {
+        if (j * TPB + tid > last) u[j] = make_uint4(NONE, NONE, NONE, NONE);
+        if (j * TPB + tid == last) r.trim(u[j], q0 + last);
+      }
     float mx = m;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (q0 + j * TPB >= r.nvec) break;
-      float v[VEC];
-      unpack<T>(u[j], v);
+      if (last >= j * TPB) {
+        float v[VEC];
+        unpack<T>(u[j], v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, v[e]);
+        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, v[e]);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // one vector's floats at a time: more of them at once only spill
     }
+    if constexpr (sizeof(T) == 2) keep_packed(u);
+    if (q0 == 0 && hit) xt = to_f(x[k]);
     const float ms = mx == -INFINITY ? 0.f : mx;
-    if (q0 > 0) lp_join(m, s, t, mx, 0.f, 0.f);
+    if (LONG && q0 > 0) lp_join(m, s, t, mx, 0.f, 0.f);
     m = mx;
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
-      if (q0 + j * TPB >= r.nvec) break;
-      float v[VEC];
-      unpack<T>(u[j], v);
+      if (last >= j * TPB) {
+        float v[VEC];
+        unpack<T>(u[j], v);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float z = (v[e] - ms) * LOG2E, p = __builtin_amdgcn_exp2f(z);
-        s += p;
-        t = fmaf(p, fmaxf(z, -200.f), t);  // p is 0 long before -200: a finite factor beside it
+        for (int e = 0; e < VEC; ++e) {
+          const float z = (v[e] - ms) * LOG2E, p = __builtin_amdgcn_exp2f(z);
+          s += p;
+          t = fmaf(p, fmaxf(z, -200.f), t);  // p is 0 long before -200: a finite factor beside it
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
   lane_max[w][lane] = m;
@@ -148,8 +169,14 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
     part[w][2] = ts;
   }
   __syncthreads();
-  float M = part[0][0], S = part[0][1], Z = part[0][2];
-  for (int i = 1; i < NW; ++i) lp_join(M, S, Z, part[i][0], part[i][1], part[i][2]);
+  float M = part[lane % NW][0], S = part[lane % NW][1], Z = part[lane % NW][2];
+#pragma unroll
+  for (int o = 1; o < NW; o <<= 1) lp_join(M, S, Z, __shfl_xor(M, o, 64), __shfl_xor(S, o, 64), __shfl_xor(Z, o, 64));
+  // the lanes join in different orders and may differ in the last bit: lane 0's holds for all, or an
+  // alternative's value would go by the place that it got in the list
+  M = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, M)));
+  S = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, S)));
+  Z = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, Z)));
   const bool none = S == 0.f;  // every logit -inf
   const float l2 = none ? 0.f : log2f(S), ls = l2 * LN2;
   if (tid == 0) {
@@ -169,31 +196,21 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
     if (__popcll(__ballot(key >= (bar | 1u << b))) >= top) bar |= 1u << b;
   const float least = bar <= 0x007fu ? -INFINITY
                                      : __builtin_bit_cast(float, bar & 0x8000u ? (bar << 16) & 0x7fffffffu : ~(bar << 16));
-  if (__any(m >= least)) {
-    for (int q0 = 0; q0 < r.nvec; q0 += TPB * NV) {
+  // a thread with such an element goes over its part of the row again: few do, and it is in the cache
+  if (m >= least)
+    for (int q = tid; q < r.nvec; q += TPB) {
+      float v[VEC];
+      unpack<T>(r.base[q], v);
 #pragma unroll
-      for (int j = 0; j < NV; ++j) {
-        const int qb = q0 + j * TPB, q = qb + tid;
-        if (qb >= r.nvec) break;
-        uint4 uu = u[j];
-        if (r.nvec > TPB * NV) {  // the registers hold the last segment alone
-          uu = none4;
-          if (q < r.nvec) uu = r.load(q);
-        }
-        float v[VEC];
-        unpack<T>(uu, v);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e)
-          if (v[e] >= least) {
-            const int c = q * VEC + e - r.skew;
-            if (c >= 0 && c < V) {
-              const int at = atomicAdd(&ncand, 1);
-              if (at < LP_CAND) cand[at] = ((uint64_t)order_key(v[e]) << 32) | (0xffffffffu - (uint32_t)c);
-            }
+      for (int e = 0; e < VEC; ++e)
+        if (v[e] >= least) {
+          const int c = q * VEC + e - r.skew;
+          if (c >= 0 && c < V) {
+            const int at = atomicAdd(&ncand, 1);
+            if (at < LP_CAND) cand[at] = ((uint64_t)order_key(v[e]) << 32) | (0xffffffffu - (uint32_t)c);
           }
-      }
+        }
     }
-  }
   __syncthreads();
   const int nc = ncand;
   if (nc >= top && nc <= LP_CAND) {
@@ -295,15 +312,16 @@ extern "C" int imgcap_token_logprobs(int dtype, int n, int V, int top, const voi
   IMGCAP_REQUIRE(logits && entropy && stats && (!targets || logp) && (top == 0 || (top_logp && top_ids)),
                  "imgcap_token_logprobs: NULL operand");
   hipStream_t st = (hipStream_t)stream;
-#define LP_(T, TPB, NV)                                                                                        \
-  hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, NV>), dim3(n), dim3(TPB), 0, st, V, top, (const T*)logits, \
-                     (long)ld, targets, logp, entropy, stats, top_logp, top_ids)
+#define LP_(T, TPB, NV, LONG)                                                                             \
+  hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, NV, LONG>), dim3(n), dim3(TPB), 0, st, V, top,        \
+                     (const T*)logits, (long)ld, targets, logp, entropy, stats, top_logp, top_ids)
 #define LP_T(T)                                               \
   do {                                                        \
     const int vec = 16 / (int)sizeof(T), nvec = (V + 2 * vec - 2) / vec; \
-    if (nvec <= 256 * 8 && n > 512) LP_(T, 256, 8);           \
-    else if (nvec <= 1024 * 8) LP_(T, 1024, 8);               \
-    else LP_(T, 1024, 16);                                    \
+    if (nvec <= 256 * 8 && n > 512) LP_(T, 256, 8, false);    \
+    else if (nvec <= 1024 * 8) LP_(T, 1024, 8, false);        \
+    else if (nvec <= 1024 * 16) LP_(T, 1024, 16, false);      \
+    else LP_(T, 1024, 8, true);                               \
   } while (0)
   if (dtype == IMGCAP_BF16) LP_T(bf16);
   else LP_T(float);
@@ -322,7 +340,7 @@ extern "C" int imgcap_token_logprobs_bwd(int dtype, int n, int V, const void* lo
   if (n == 0) return 0;
   IMGCAP_REQUIRE(logits && stats && entropy && dlogits && (!dlogp || targets),
                  "imgcap_token_logprobs_bwd: NULL operand");
-  IMGCAP_REQUIRE(logits != dlogits || ld == ldd, "imgcap_token_logprobs_bwd: in place needs equal pitches");
+  IMGCAP_REQUIRE(logits != dlogits || ld == ldd || n == 1, "imgcap_token_logprobs_bwd: in place needs equal pitches");
   hipStream_t st = (hipStream_t)stream;
 #define LPB_(T)                                                                                                     \
   do {                                                                                                              \

@@ -8,32 +8,14 @@
 namespace imgcap {
 
 // ---- page planning ------------------------------------------------------------------------
-// One workgroup walks the requests in chunks of its width: integer prefix sums give each request
-// its place on the stack of free pages and its first token, then every token finds its request by
-// bisection of the starts.  All sums are 64-bit: lengths are the caller's and may be anything.
-DEV long wave_scan_incl(long v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) {
-    const long u = __shfl_up(v, o, 64);
-    if ((int)(threadIdx.x & 63) >= o) v += u;
-  }
-  return v;
-}
-// inclusive prefix over the block; `total` gets the block's sum.  red: blockDim / 64 longs.
-DEV long block_scan_incl(long v, long* red, long& total) {
-  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
-  v = wave_scan_incl(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 63) red[w] = v;
-  __syncthreads();
-  long before = 0, all = 0;
-  for (int i = 0; i < nw; ++i) {
-    if (i < w) before += red[i];
-    all += red[i];
-  }
-  total = all;
-  return v + before;
-}
+// Integer prefix sums give each request its place on the stack of free pages and its first token;
+// every token then finds its request by bisection of the starts.  A step of up to PLAN_ROWS requests
+// is one pass of one workgroup with 32-bit sums in the lanes; up to PLAN_TOKENS tokens it also lays
+// out the tokens itself, from LDS.  It is latency that counts there: lengths, count and the page that
+// a request has open are loaded at once, one more dependent load follows (the page taken off the
+// stack).  More tokens go to a second launch over the whole chip; more requests (or sums that might
+// pass 32 bits) to a pass in chunks with 64-bit sums.
+constexpr int PLAN_ROWS = 1024, PLAN_TOKENS = 4096, PLAN_CAP = 1 << 20;
 
 struct PlanArgs {
   int B, width, lp, pool, tokens;
@@ -53,39 +35,142 @@ struct PlanArgs {
   int32_t* ws;  // [B] first page of each request on the stack, [B] = the stack's top
 };
 
-// token i of the step: its request, position and slot; the token that opens a page enters the page
-// into the table
-DEV void plan_token(const PlanArgs& a, int i, int total, const int32_t* starts, const int32_t* first, int top) {
-  if (i >= total) {
-    a.slots[i] = -1;
-    a.rows[i] = -1;
-    a.positions[i] = 0;
-    return;
+DEV int wave_scan_incl(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15: row 0 -> 1, 2 -> 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast 31: rows 0, 1 -> 2, 3
+  return v;
+}
+DEV long wave_scan_incl(long v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const long u = __shfl_up(v, o, 64);
+    if ((int)(threadIdx.x & 63) >= o) v += u;
   }
-  int lo = 0, hi = a.B;  // starts[lo] <= i < starts[hi]
+  return v;
+}
+// inclusive prefix over the block; `total` gets the block's sum.  red: blockDim / 64 values.
+template <typename I> DEV I block_scan_incl(I v, I* red, I& total) {
+  const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
+  v = wave_scan_incl(v);
+  if (nw == 1) {
+    total = __shfl(v, 63, 64);
+    return v;
+  }
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) red[w] = v;
+  __syncthreads();
+  I before = 0, all = 0;
+  for (int i = 0; i < nw; ++i) {
+    if (i < w) before += red[i];
+    all += red[i];
+  }
+  total = all;
+  return v + before;
+}
+
+// the request of token i: starts[r] <= i < starts[r + 1] (n requests)
+DEV int plan_row(const int32_t* starts, int n, int i) {
+  int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (starts[mid] <= i) lo = mid;
     else hi = mid;
   }
-  const int past = a.past[lo], page = 1 << a.lp;
-  const long pos = (long)past + (i - starts[lo]);
-  const int pi = (int)(pos >> a.lp), off = (int)pos & (page - 1);
-  const int have = (int)(((long)past + page - 1) >> a.lp);
-  int32_t* entry = a.table + (long)lo * a.table_row + pi;
-  int id;
-  if (pi < have) {
-    id = *entry;
-  } else {
-    id = a.free_ids[top - 1 - first[lo] - (pi - have)];
-    if (off == 0) *entry = id;
-  }
+  return lo;
+}
+DEV void plan_put(const PlanArgs& a, int i, int row, long pos, int id) {
+  const int off = (int)pos & ((1 << a.lp) - 1);
   a.slots[i] = (unsigned)id < (unsigned)a.pool ? ((int64_t)id << a.lp) + off : -1;
-  a.rows[i] = lo;
+  a.rows[i] = row;
   a.positions[i] = pos;
 }
+DEV void plan_none(const PlanArgs& a, int i) {
+  a.slots[i] = -1;
+  a.rows[i] = -1;
+  a.positions[i] = 0;
+}
+// the id of page pi of a request that holds `have` pages and takes the next ones from place `at` of
+// the stack down; the token that opens a page enters it into the table
+DEV int plan_page(const PlanArgs& a, int row, int pi, int have, int at, long pos) {
+  const int id = a.free_ids[at - (pi - have)];
+  if (((int)pos & ((1 << a.lp) - 1)) == 0) a.table[(long)row * a.table_row + pi] = id;
+  return id;
+}
 
-__global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand) {
+__global__ __launch_bounds__(PLAN_ROWS) void paged_plan_kernel(PlanArgs a, int expand) {
+  __shared__ int red[16];
+  __shared__ int starts_s[PLAN_ROWS + 1], at_s[PLAN_ROWS], past_s[PLAN_ROWS], open_s[PLAN_ROWS];
+  const int T = blockDim.x, b = threadIdx.x, page = 1 << a.lp;
+  const bool in = b < a.B;
+  const int past = in ? a.past[b] : 0, add = in ? a.add[b] : -1;
+  int top = min(max(*a.count, 0), a.pool);
+  const long lp = past, la = add, room = (long)a.width << a.lp;
+  const bool live = add >= 0;
+  const int have = (int)((max(lp, 0l) + page - 1) >> a.lp);
+  int open = -1;  // the page that the request's next token goes to, if it has one open
+  if (live && past > 0 && (past & (page - 1)) && (past >> a.lp) < a.width) open = a.table[b * a.table_row + (past >> a.lp)];
+  const int back = in && !live ? min(have, a.width) : 0;
+  bool fits = live && past >= 0 && lp + la <= room;
+  const int asked = fits ? min(add, a.tokens + 1) : 0;  // one past the capacity is as far as it counts
+  int asked_all, need_all, back_all = 0;
+  const int tok = block_scan_incl(asked, red, asked_all);
+  fits = fits && tok <= a.tokens;
+  const int need = fits ? (int)((lp + la + page - 1) >> a.lp) - have : 0;
+  const int upto = block_scan_incl(need, red, need_all);
+  if (__syncthreads_or(back > 0)) {  // pages of ended requests go back on the stack, in the requests' order
+    const int before = block_scan_incl(back, red, back_all) - back;
+    starts_s[b] = back;
+    at_s[b] = before;
+    __syncthreads();
+    for (int r = b >> 6; r < a.B; r += T >> 6)
+      for (int j = b & 63; j < starts_s[r]; j += 64)
+        if ((long)top + at_s[r] + j < a.pool) a.free_ids[top + at_s[r] + j] = a.table[r * a.table_row + j];
+    __syncthreads();
+    top = (int)min((long)top + back_all, (long)a.pool);
+  }
+  const bool granted = fits && (need == 0 || upto <= top);
+  int start = tok - asked, total = asked_all, used = need_all;
+  if (asked_all > a.tokens || need_all > top) {  // some request waits: what the others get, again
+    start = block_scan_incl(granted ? add : 0, red, total) - (granted ? add : 0);
+    block_scan_incl(granted ? need : 0, red, used);
+  }
+  if (in) {
+    a.lens[b] = live ? past + (granted ? add : 0) : 0;
+    a.starts[b] = start;
+    a.waits[b] = live && !granted ? 1 : 0;
+  }
+  if (b == 0) {
+    a.starts[a.B] = total;
+    *a.count_out = top - used;
+  }
+  if (!expand) {
+    if (in) a.ws[b] = upto - need;
+    if (b == 0) a.ws[a.B] = top;
+    return;
+  }
+  starts_s[b] = start;
+  at_s[b] = top - 1 - (upto - need);
+  past_s[b] = past;
+  open_s[b] = open;
+  __syncthreads();
+  for (int i = b; i < a.tokens; i += T) {
+    if (i >= total) {
+      plan_none(a, i);
+      continue;
+    }
+    const int r = plan_row(starts_s, a.B, i), p0 = past_s[r];
+    const long pos = (long)p0 + (i - starts_s[r]);
+    const int pi = (int)(pos >> a.lp), h = (int)(((long)p0 + page - 1) >> a.lp);
+    plan_put(a, i, r, pos, pi < h ? open_s[r] : plan_page(a, r, pi, h, at_s[r], pos));
+  }
+}
+
+// any number of requests: chunks of the workgroup's width, 64-bit sums
+__global__ __launch_bounds__(1024) void paged_plan_long_kernel(PlanArgs a) {
   __shared__ long red[16];
   __shared__ long base_s[1024];
   __shared__ int back_s[1024];
@@ -93,7 +178,6 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand
   const int page = 1 << a.lp;
   const long room = (long)a.width << a.lp;
   long top = min(max(*a.count, 0), a.pool);
-  // pages of ended requests go back on the stack, in the requests' order
   for (int b0 = 0; b0 < a.B; b0 += T) {
     const int b = b0 + tid;
     long back = 0;
@@ -119,7 +203,7 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand
     const bool live = add >= 0;
     bool fits = live && past >= 0 && past + add <= room;
     long total;
-    const long tok = tok0 + block_scan_incl(fits ? add : 0, red, total);
+    const long tok = tok0 + block_scan_incl(fits ? add : 0l, red, total);
     tok0 += total;
     fits = fits && tok <= a.tokens;
     const long have = (max(past, 0l) + page - 1) >> a.lp;
@@ -127,9 +211,9 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand
     const long upto = page0 + block_scan_incl(need, red, total);
     page0 += total;
     const bool granted = fits && (need == 0 || upto <= top);
-    const long out = out0 + block_scan_incl(granted ? add : 0, red, total);
+    const long out = out0 + block_scan_incl(granted ? add : 0l, red, total);
     out0 += total;
-    block_scan_incl(granted ? need : 0, red, total);
+    block_scan_incl(granted ? need : 0l, red, total);
     used += total;
     if (in) {
       a.lens[b] = live ? (int)(past + (granted ? add : 0)) : 0;
@@ -143,14 +227,32 @@ __global__ __launch_bounds__(1024) void paged_plan_kernel(PlanArgs a, int expand
     a.ws[a.B] = (int)top;
     *a.count_out = (int)(top - used);
   }
-  if (!expand) return;
-  __syncthreads();
-  for (int i = tid; i < a.tokens; i += T) plan_token(a, i, (int)out0, a.starts, a.ws, (int)top);
 }
 
+// lays out the tokens after either planner: SLOT_TOKENS a workgroup, the starts in LDS if they fit
+constexpr int SLOT_TOKENS = 1024, SLOT_ROWS = 4096;
 __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
-  const int i = blockIdx.x * 256 + threadIdx.x;
-  if (i < a.tokens) plan_token(a, i, a.starts[a.B], a.starts, a.ws, a.ws[a.B]);
+  __shared__ int32_t starts_s[SLOT_ROWS];
+  const int32_t* starts = a.starts;
+  if (a.B <= SLOT_ROWS) {
+    for (int i = threadIdx.x; i < a.B; i += 256) starts_s[i] = a.starts[i];
+    __syncthreads();
+    starts = starts_s;
+  }
+  const int total = a.starts[a.B], top = a.ws[a.B], page = 1 << a.lp;
+#pragma unroll
+  for (int j = 0; j < SLOT_TOKENS / 256; ++j) {
+    const long i = (long)blockIdx.x * SLOT_TOKENS + 256 * j + threadIdx.x;
+    if (i >= a.tokens) break;
+    if (i >= total) {
+      plan_none(a, (int)i);
+      continue;
+    }
+    const int r = plan_row(starts, a.B, (int)i), p0 = a.past[r];
+    const long pos = (long)p0 + (i - starts[r]);
+    const int pi = (int)(pos >> a.lp), h = (int)(((long)p0 + page - 1) >> a.lp);
+    plan_put(a, (int)i, r, pos, pi < h ? a.table[r * a.table_row + pi] : plan_page(a, r, pi, h, top - 1 - a.ws[r], pos));
+  }
 }
 
 // ---- cache writer -------------------------------------------------------------------------
@@ -507,16 +609,24 @@ extern "C" int imgcap_paged_plan(int B, int width, int page, int pool, int token
   IMGCAP_REQUIRE(is_pow2(page) && page <= 1024, "imgcap_paged_plan: page must be a power of two, at most 1024");
   IMGCAP_REQUIRE((int64_t)width * page < (1ll << 31), "imgcap_paged_plan: width * page must be below 2^31");
   IMGCAP_REQUIRE(table_row >= width, "imgcap_paged_plan: table rows overlap");
-  IMGCAP_REQUIRE(past && add && table && free_ids && count && count_out && lens && starts && waits && ws &&
+  IMGCAP_REQUIRE(past && add && table && free_ids && count && count_out && lens && starts && waits &&
                      (tokens == 0 || (slots && rows && positions)),
                  "imgcap_paged_plan: NULL operand");
   const PlanArgs a{B, width, log2_of(page), pool, tokens, past, add, table, (long)table_row, free_ids, count, count_out,
                    lens, starts, slots, rows, positions, waits, ws};
-  const int threads = B >= 1024 || tokens >= 1024 ? 1024 : ((B > tokens ? B : tokens) + 63) / 64 * 64;
-  const bool one = tokens <= 4096;
-  hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(threads), 0, (hipStream_t)stream, a, one ? 1 : 0);
-  if (!one)
-    hipLaunchKernelGGL(paged_slots_kernel, dim3((tokens + 255) / 256), dim3(256), 0, (hipStream_t)stream, a);
+  const bool fast = B <= PLAN_ROWS && tokens <= PLAN_CAP && width <= PLAN_CAP;
+  const bool one = fast && tokens <= PLAN_TOKENS;
+  IMGCAP_REQUIRE(one || ws, "imgcap_paged_plan: NULL workspace");
+  hipStream_t st = (hipStream_t)stream;
+  if (fast) {
+    const int most = one && tokens > B ? (tokens < PLAN_ROWS ? tokens : PLAN_ROWS) : B;
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3((most + 63) / 64 * 64), 0, st, a, one ? 1 : 0);
+  } else {
+    hipLaunchKernelGGL(paged_plan_long_kernel, dim3(1), dim3(1024), 0, st, a);
+  }
+  if (!one && tokens > 0)
+    hipLaunchKernelGGL(paged_slots_kernel, dim3((unsigned)(((int64_t)tokens + SLOT_TOKENS - 1) / SLOT_TOKENS)), dim3(256),
+                       0, st, a);
   IMGCAP_CHECK_LAUNCH("imgcap_paged_plan");
   return 0;
 }

@@ -615,33 +615,51 @@ def transpose(x, out=None):
 
 
 # ---- paged key/value cache and token log-probabilities ------------------------------------------
+# These are calls of a few microseconds on the GPU, one after another in a decoding loop, so the
+# host side is kept to plain integers: devices as indices, the raw stream handle (0.1 us; a Stream
+# object costs 2.6), no library workspace looked after (they take none).
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
 def _one_device(name, *ts):
-    """The GPU that all of ``ts`` (None left out) live on."""
-    dev = ts[0].device
-    if dev.type != "cuda":
+    """Index of the GPU that all of ``ts`` (None left out) live on."""
+    dev = ts[0].get_device()
+    if dev < 0:
         raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name}: tensors on {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
     return dev
 
 
 def _call_on(dev, name, *args):
-    """``name`` on the current stream of ``dev``, whichever device is the current one."""
-    if dev.index == torch.cuda.current_device():
-        _abi.call(name, *args, stream())
-    else:
-        with torch.cuda.device(dev):
-            _abi.call(name, *args, stream())
+    """Return code of ``name`` on the current stream of GPU ``dev``, whichever is the current one."""
+    fn = getattr(_abi.lib(), name)
+    if dev == torch.cuda.current_device():
+        return fn(*args, _raw_stream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, _raw_stream(dev))
 
 
 def _want(name, what, t, dtype, shape, contiguous=True):
     if t.dtype != dtype:
         raise TypeError(f"{name}: {what} must be {dtype}, got {t.dtype}")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name}: {what} must have shape {shape}, got {tuple(t.shape)}")
     if contiguous and not t.is_contiguous():
         raise ValueError(f"{name}: {what} must be contiguous")
+
+
+def _int_rows(name, what, t, rows):
+    """(row stride, width) of an int32 matrix of ``rows`` rows with unit inner stride."""
+    if t.dim() != 2 or t.dtype != torch.int32 or t.shape[0] != rows or t.stride(1) != 1:
+        raise ValueError(f"{name}: {what} must be [{rows}, width] int32 with unit inner stride")
+    width = t.shape[1]
+    return (t.stride(0) if rows > 1 else width), width
+
+
+# where one workgroup plans a whole step and needs no scratch (paged.hip PLAN_ROWS, PLAN_TOKENS, PLAN_CAP)
+_PLAN_ROWS, _PLAN_TOKENS, _PLAN_CAP = 1024, 4096, 1 << 20
 
 
 def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, out=None):
@@ -654,61 +672,74 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     [tokens] int32, positions [tokens] int64, waits [B] int32); pass it back as ``out`` to have it
     filled again (a captured graph's outputs).  A request that does not fit -- lengths past the table,
     no page left, no token left -- waits: waits[b] = 1, nothing else of it changes."""
+    name = "paged_plan"
     count_out = count if count_out is None else count_out
-    dev = _one_device("paged_plan", past, new, table, free, count, count_out)
-    if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
-        raise ValueError("paged_plan: table must be [B, width] int32 with unit inner stride")
-    B, width = table.shape
-    _want("paged_plan", "past", past, torch.int32, (B,))
-    _want("paged_plan", "new", new, torch.int32, (B,))
-    _want("paged_plan", "free", free, torch.int32, (free.numel(),))
-    _want("paged_plan", "count", count, torch.int32, (1,))
-    _want("paged_plan", "count_out", count_out, torch.int32, (1,))
+    dev = _one_device(name, past, new, table, free, count, count_out)
+    B = past.numel()
+    table_row, width = _int_rows(name, "table", table, B)
+    i32, i64 = torch.int32, torch.int64
+    _want(name, "past", past, i32, (B,))
+    _want(name, "new", new, i32, (B,))
+    _want(name, "free", free, i32, (free.numel(),))
+    _want(name, "count", count, i32, (1,))
+    _want(name, "count_out", count_out, i32, (1,))
     if out is None:
-        i32, i64 = dict(device=dev, dtype=torch.int32), dict(device=dev, dtype=torch.int64)
-        out = (torch.empty(B, **i32), torch.empty(B + 1, **i32), torch.empty(tokens, **i64),
-               torch.empty(tokens, **i32), torch.empty(tokens, **i64), torch.empty(B, **i32))
+        if tokens < 0:
+            raise ValueError(f"paged_plan: tokens must not be negative, got {tokens}")
+        out = (past.new_empty(B), past.new_empty(B + 1), past.new_empty(tokens, dtype=i64), past.new_empty(tokens),
+               past.new_empty(tokens, dtype=i64), past.new_empty(B))
+        lens, starts, slots, rows, positions, waits = out
     else:
-        _one_device("paged_plan", past, *out)
-        for what, t, dtype, n in zip(("lens", "starts", "slots", "rows", "positions", "waits"), out,
-                                     (torch.int32, torch.int32, torch.int64, torch.int32, torch.int64, torch.int32),
-                                     (B, B + 1, tokens, tokens, tokens, B)):
-            _want("paged_plan", what, t, dtype, (n,))
-    lens, starts, slots, rows, positions, waits = out
-    ws = torch.empty(B + 1, device=dev, dtype=torch.int32)
-    _call_on(dev, "imgcap_paged_plan", B, width, page, free.numel(), tokens, past.data_ptr(), new.data_ptr(),
-             table.data_ptr(), table.stride(0) if B > 1 else width, free.data_ptr(), count.data_ptr(),
-             count_out.data_ptr(), lens.data_ptr(), starts.data_ptr(), slots.data_ptr(), rows.data_ptr(),
-             positions.data_ptr(), waits.data_ptr(), ws.data_ptr())
+        lens, starts, slots, rows, positions, waits = out
+        _one_device(name, past, *out)
+        _want(name, "lens", lens, i32, (B,))
+        _want(name, "starts", starts, i32, (B + 1,))
+        _want(name, "slots", slots, i64, (tokens,))
+        _want(name, "rows", rows, i32, (tokens,))
+        _want(name, "positions", positions, i64, (tokens,))
+        _want(name, "waits", waits, i32, (B,))
+    ws = None if B <= _PLAN_ROWS and tokens <= _PLAN_TOKENS and width <= _PLAN_CAP else past.new_empty(B + 1)
+    rc = _call_on(dev, "imgcap_paged_plan", B, width, page, free.numel(), tokens, past.data_ptr(), new.data_ptr(),
+                  table.data_ptr(), table_row, free.data_ptr(), count.data_ptr(), count_out.data_ptr(), lens.data_ptr(),
+                  starts.data_ptr(), slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), waits.data_ptr(), ptr(ws))
+    if rc:
+        _abi.fail("imgcap_paged_plan", rc)
     return out
 
 
 def _cache_pair(name, k, v):
     if k.dim() != 4 or k.shape != v.shape:
         raise ValueError(f"{name}: caches must be [pages, page, kv heads, head dim], both alike")
-    if k.stride(3) != 1 or v.stride(3) != 1:
+    ks, vs = k.stride(), v.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError(f"{name}: caches must have unit inner stride")
-    return k.shape
+    return k.shape, ks, vs
 
 
 def paged_write(k, v, k_cache, v_cache, slots):
     """k_cache[slot // page, slot % page] = k[i] for slot = slots[i] (int64, imgcap_paged_write), and
     the values alike: k / v [n, kv heads, head dim] views, caches [pages, page, kv heads, head dim] of
     any strides.  A slot outside the cache (-1: padding) is skipped.  Slots of one call are distinct."""
-    dev = _one_device("paged_write", k, v, k_cache, v_cache, slots)
-    pages, page, heads, dh = _cache_pair("paged_write", k_cache, v_cache)
+    name = "paged_write"
+    dev = _one_device(name, k, v, k_cache, v_cache, slots)
+    (pages, page, heads, dh), kc, vc = _cache_pair(name, k_cache, v_cache)
     if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
         raise TypeError("paged_write: k, v and the caches must share a dtype")
     n = slots.numel()
-    _want("paged_write", "slots", slots, torch.int64, (n,))
-    if tuple(k.shape) != (n, heads, dh) or tuple(v.shape) != (n, heads, dh):
+    _want(name, "slots", slots, torch.int64, (n,))
+    if k.shape != (n, heads, dh) or v.shape != (n, heads, dh):
         raise ValueError(f"paged_write: k and v must be [{n}, {heads}, {dh}]")
-    if n and (k.stride(2) != 1 or v.stride(2) != 1):
+    if n == 0:
+        return
+    ks, vs = k.stride(), v.stride()
+    if ks[2] != 1 or vs[2] != 1:
         raise ValueError("paged_write: k and v must have unit inner stride")
-    d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-                            *k_cache.stride()[:3], *v_cache.stride()[:3], k.data_ptr(), v.data_ptr(),
-                            k_cache.data_ptr(), v_cache.data_ptr(), slots.data_ptr())
-    _call_on(dev, "imgcap_paged_write", ctypes.byref(d))
+    d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0],
+                            vc[1], vc[2], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                            slots.data_ptr())
+    rc = _call_on(dev, "imgcap_paged_write", d)
+    if rc:
+        _abi.fail("imgcap_paged_write", rc)
 
 
 def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=None, out=None, lse=None):
@@ -718,39 +749,51 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
     ``max_len`` (default: the table's width) bounds the lengths from the host; the work is cut for it.
     A request of length 0 gets zeros; positions on a page outside the cache are not there.
     ``lse`` [B, H] fp32 gets the natural log-sum-exp of the scores (default scale: head dim ** -0.5)."""
-    dev = _one_device("paged_attention", q, k_cache, v_cache, table, lens, out, lse)
-    pages, page, hkv, dh = _cache_pair("paged_attention", k_cache, v_cache)
+    name = "paged_attention"
+    dev = _one_device(name, q, k_cache, v_cache, table, lens, out, lse)
+    (pages, page, hkv, dh), ks, vs = _cache_pair(name, k_cache, v_cache)
     if q.dim() != 3 or q.shape[2] != dh:
         raise ValueError(f"paged_attention: q must be [B, H, {dh}]")
     if not (q.dtype == k_cache.dtype == v_cache.dtype):
         raise TypeError("paged_attention: q and the caches must share a dtype")
-    B, H = q.shape[:2]
-    if table.dim() != 2 or table.dtype != torch.int32 or table.shape[0] != B or table.stride(1) != 1:
-        raise ValueError("paged_attention: table must be [B, width] int32 with unit inner stride")
-    _want("paged_attention", "lens", lens, torch.int32, (B,))
+    B, H, _ = q.shape
+    table_row, width = _int_rows(name, "table", table, B)
+    _want(name, "lens", lens, torch.int32, (B,))
     if out is None:
-        out = torch.empty(B, H, dh, device=dev, dtype=q.dtype)
+        out = q.new_empty((B, H, dh))
     else:
-        _want("paged_attention", "out", out, q.dtype, (B, H, dh), contiguous=False)
-    if q.stride(2) != 1 or out.stride(2) != 1:
+        _want(name, "out", out, q.dtype, (B, H, dh), contiguous=False)
+    qs, os_ = q.stride(), out.stride()
+    if qs[2] != 1 or os_[2] != 1:
         raise ValueError("paged_attention: q and out must have unit inner stride")
     if lse is not None:
-        _want("paged_attention", "lse", lse, torch.float32, (B, H))
+        _want(name, "lse", lse, torch.float32, (B, H))
     if B == 0:
         return out
-    width = table.shape[1]
     d = _abi.PagedAttnDesc(dt(q), B, H, hkv, dh, page, pages, width, width * page if max_len is None else max_len,
-                           dh ** -0.5 if scale is None else scale, q.stride(0), q.stride(1), out.stride(0),
-                           out.stride(1), *k_cache.stride()[:3], *v_cache.stride()[:3], table.stride(0), q.data_ptr(),
-                           k_cache.data_ptr(), v_cache.data_ptr(), out.data_ptr(), ptr(lse), table.data_ptr(),
-                           lens.data_ptr(), None, 0)
-    need = ctypes.c_int64(0)
-    _abi.check("imgcap_paged_attention_ws", ctypes.byref(d), ctypes.byref(need))
-    if need.value:  # a split length: the parts' maxima, sums and outputs
-        ws = torch.empty(need.value, device=dev, dtype=torch.uint8)
+                           dh ** -0.5 if scale is None else scale, qs[0], qs[1], os_[0], os_[1], ks[0], ks[1], ks[2],
+                           vs[0], vs[1], vs[2], table_row, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                           out.data_ptr(), ptr(lse), table.data_ptr(), lens.data_ptr(), None, 0)
+    rc = _call_on(dev, "imgcap_paged_attention", d)
+    if rc == _abi.IMGCAP_EWORKSPACE:  # a split length: the parts' maxima, sums and outputs; nothing ran yet
+        need = ctypes.c_int64(0)
+        _abi.check("imgcap_paged_attention_ws", d, need)
+        ws = q.new_empty(need.value, dtype=torch.uint8)
         d.ws, d.ws_bytes = ws.data_ptr(), need.value
-    _call_on(dev, "imgcap_paged_attention", ctypes.byref(d))
+        rc = _call_on(dev, "imgcap_paged_attention", d)
+    if rc:
+        _abi.fail("imgcap_paged_attention", rc)
     return out
+
+
+def _logit_rows(name, logits, V):
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        raise ValueError(f"{name}: logits must be [n, V] with unit inner stride")
+    n, cols = logits.shape
+    V = cols if V is None else V
+    if not 0 < V <= cols:
+        raise ValueError(f"{name}: V must be in 1 .. {cols}")
+    return n, V, (logits.stride(0) if n > 1 else cols)
 
 
 def token_logprobs(logits, targets=None, V=None, *, top=0):
@@ -760,21 +803,22 @@ def token_logprobs(logits, targets=None, V=None, *, top=0):
     [n, 2] fp32 for token_logprobs_bwd, top_logp [n, top] fp32, top_ids [n, top] int64).  A target
     outside [0, V) (-1: padding) gives logp 0.  Alternatives come in falling order, equal ones by
     index, NaN last.  Logits of -inf have no weight; a row of them alone gives -inf and entropy 0."""
-    dev = _one_device("token_logprobs", logits, targets)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("token_logprobs: logits must be [n, V] with unit inner stride")
-    n = logits.shape[0]
-    V = logits.shape[1] if V is None else V
-    if not 0 < V <= logits.shape[1]:
-        raise ValueError(f"token_logprobs: V must be in 1 .. {logits.shape[1]}")
+    name = "token_logprobs"
+    dev = _one_device(name, logits, targets)
+    n, V, ld = _logit_rows(name, logits, V)
+    f32 = torch.float32
+    if not 0 <= top <= min(64, V):
+        raise ValueError(f"token_logprobs: top must be in 0 .. {min(64, V)}")
+    logp = None
     if targets is not None:
-        _want("token_logprobs", "targets", targets, torch.int64, (n,))
-    f32 = dict(device=dev, dtype=torch.float32)
-    logp = None if targets is None else torch.empty(n, **f32)
-    entropy, stats, top_logp = torch.empty(n, **f32), torch.empty(n, 2, **f32), torch.empty(n, top, **f32)
-    top_ids = torch.empty(n, top, device=dev, dtype=torch.int64)
-    _call_on(dev, "imgcap_token_logprobs", dt(logits), n, V, top, logits.data_ptr(), logits.stride(0), ptr(targets),
-             ptr(logp), entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+        _want(name, "targets", targets, torch.int64, (n,))
+        logp = logits.new_empty(n, dtype=f32)
+    entropy, stats = logits.new_empty(n, dtype=f32), logits.new_empty((n, 2), dtype=f32)
+    top_logp, top_ids = logits.new_empty((n, top), dtype=f32), logits.new_empty((n, top), dtype=torch.int64)
+    rc = _call_on(dev, "imgcap_token_logprobs", dt(logits), n, V, top, logits.data_ptr(), ld, ptr(targets), ptr(logp),
+                  entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+    if rc:
+        _abi.fail("imgcap_token_logprobs", rc)
     return logp, entropy, stats, top_logp, top_ids
 
 
@@ -782,29 +826,36 @@ def token_logprobs_bwd(logits, targets, stats, entropy, dlogp=None, dentropy=Non
     """Gradient of the logits of token_logprobs from those of logp and entropy ([n] fp32, either may
     be None) -> dlogits [n, V] in the logits' dtype (of a given ``dlogits`` [n, >= V], which may be
     ``logits`` itself, the columns from V on stay).  The alternatives have no gradient."""
-    dev = _one_device("token_logprobs_bwd", logits, targets, stats, entropy, dlogp, dentropy, dlogits)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        raise ValueError("token_logprobs_bwd: logits must be [n, V] with unit inner stride")
-    n = logits.shape[0]
-    V = logits.shape[1] if V is None else V
-    if not 0 < V <= logits.shape[1]:
-        raise ValueError(f"token_logprobs_bwd: V must be in 1 .. {logits.shape[1]}")
+    name = "token_logprobs_bwd"
+    dev = _one_device(name, logits, targets, stats, entropy, dlogp, dentropy, dlogits)
+    n, V, ld = _logit_rows(name, logits, V)
+    f32 = torch.float32
     if dlogp is not None and targets is None:
         raise ValueError("token_logprobs_bwd: dlogp needs the targets")
     if targets is not None:
-        _want("token_logprobs_bwd", "targets", targets, torch.int64, (n,))
-    _want("token_logprobs_bwd", "stats", stats, torch.float32, (n, 2))
-    for what, t in (("entropy", entropy), ("dlogp", dlogp), ("dentropy", dentropy)):
-        if t is not None:
-            _want("token_logprobs_bwd", what, t, torch.float32, (n,))
+        _want(name, "targets", targets, torch.int64, (n,))
+    _want(name, "stats", stats, f32, (n, 2))
+    _want(name, "entropy", entropy, f32, (n,))
+    if dlogp is not None:
+        _want(name, "dlogp", dlogp, f32, (n,))
+    if dentropy is not None:
+        _want(name, "dentropy", dentropy, f32, (n,))
     if dlogits is None:
         vec = 16 // logits.element_size()  # rows on whole 16-byte vectors
-        dlogits = torch.empty(n, (V + vec - 1) // vec * vec, device=dev, dtype=logits.dtype)[:, :V]
-    elif dlogits.dtype != logits.dtype or dlogits.dim() != 2 or dlogits.shape[0] != n or dlogits.shape[1] < V \
-            or dlogits.stride(1) != 1:
-        raise ValueError("token_logprobs_bwd: dlogits must be [n, >= V] in the logits' dtype with unit inner stride")
-    _call_on(dev, "imgcap_token_logprobs_bwd", dt(logits), n, V, logits.data_ptr(), logits.stride(0), ptr(targets),
-             stats.data_ptr(), entropy.data_ptr(), ptr(dlogp), ptr(dentropy), dlogits.data_ptr(), dlogits.stride(0))
+        pitch = (V + vec - 1) // vec * vec
+        dlogits = logits.new_empty((n, pitch))
+        if pitch > V:
+            dlogits = dlogits[:, :V]
+    else:
+        if dlogits.dtype != logits.dtype:
+            raise TypeError("token_logprobs_bwd: dlogits must have the logits' dtype")
+        m, cols, pitch = _logit_rows(name, dlogits, None)
+        if m != n or cols < V:
+            raise ValueError(f"token_logprobs_bwd: dlogits must be [{n}, >= {V}]")
+    rc = _call_on(dev, "imgcap_token_logprobs_bwd", dt(logits), n, V, logits.data_ptr(), ld, ptr(targets),
+                  stats.data_ptr(), entropy.data_ptr(), ptr(dlogp), ptr(dentropy), dlogits.data_ptr(), pitch)
+    if rc:
+        _abi.fail("imgcap_token_logprobs_bwd", rc)
     return dlogits
 
 

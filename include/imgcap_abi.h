@@ -524,7 +524,7 @@ int imgcap_sort_gather_rows(int dtype, int B, int P, int E, int L, const int64_t
  *   lens[B] = past + granted tokens (0: ended), starts[B + 1] = prefix sums of the granted tokens;
  *   token i of the step: slots[i], rows[i] its request, positions[i]; behind the last one -1, -1, 0,
  *   and slot -1 where the page's id is outside [0, pool).
- *   ws: B + 1 int32 of scratch.  Requests must not share the pages that one of them gives back. */
+ *   ws: B + 1 int32 of scratch (NULL where B <= 1024, tokens <= 4096 and width <= 2^20).  Requests must not share the pages that one of them gives back. */
 int imgcap_paged_plan(int B, int width, int page, int pool, int tokens, const int32_t* past, const int32_t* add,
                       int32_t* table, int64_t table_row, int32_t* free_ids, const int32_t* count,
                       int32_t* count_out, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* rows,

@@ -79,7 +79,9 @@ _PLAN = dict(B=2, width=4, page=16, pool=8, tokens=2, past=A, add=A, table=A, ta
 @pytest.mark.parametrize("kw,why", [
     (dict(B=0), "positive"), (dict(width=0), "positive"), (dict(pool=0), "positive"), (dict(tokens=-1), "positive"),
     (dict(page=3), "power of two"), (dict(page=4096), "power of two"), (dict(width=1 << 28, table_row=1 << 28), "2^31"),
-    (dict(table_row=3), "overlap"), (dict(past=None), "NULL"), (dict(ws=None), "NULL"), (dict(slots=None), "NULL"),
+    (dict(table_row=3), "overlap"), (dict(past=None), "NULL"), (dict(slots=None), "NULL"),
+    (dict(ws=None, tokens=4097), "NULL"), (dict(ws=None, B=1025), "NULL"),
+    (dict(ws=None, width=(1 << 20) + 1, table_row=(1 << 20) + 1), "NULL"),
 ])
 def test_plan_refuses(kw, why):
     assert _abi.lib().imgcap_paged_plan(*{**_PLAN, **kw}.values(), None) == -1
