@@ -70,119 +70,122 @@ template <typename T> DEV void unpack(const uint4& u, float (&v)[16 / sizeof(T)]
   }
 }
 
-// The packed words stay what is kept between two passes over a row: without this the compiler keeps
-// the first pass's unpacked floats instead, twice the registers, and spills.
-template <int NV> DEV void keep_packed(uint4 (&u)[NV]) {
-#pragma unroll
-  for (int j = 0; j < NV; ++j) asm volatile("" : "+v"(u[j].x), "+v"(u[j].y), "+v"(u[j].z), "+v"(u[j].w));
+// wave-wide maximum / sum on lane-permuting moves (row_shr 1, 2, 4, 8 within 16 lanes, then
+// row_bcast 15 and 31): the result of lane 63, the same for all
+template <typename F> DEV float wave_fold(float v, float none, F f) {
+#define LP_STEP(ctrl, rows)                                                                                            \
+  v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),                        \
+                                                                 __builtin_bit_cast(int, v), ctrl, rows, 0xf, false)))
+  LP_STEP(0x111, 0xf);
+  LP_STEP(0x112, 0xf);
+  LP_STEP(0x114, 0xf);
+  LP_STEP(0x118, 0xf);
+  LP_STEP(0x142, 0xa);
+  LP_STEP(0x143, 0xc);
+#undef LP_STEP
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+DEV float wave_all_max(float v) {
+  return wave_fold(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
+}
+DEV float wave_all_sum(float v) {
+  return wave_fold(v, 0.f, [](float a, float b) { return a + b; });
+}
+// the lanes' parts (reference c, -inf: nothing yet; sum s, weighted sum t) as one, in every lane; a
+// difference that passes the float range weighs nothing
+DEV void lp_join_lanes(float& c, float& s, float& t) {
+  const float C = wave_all_max(c), cs = C == -INFINITY ? 0.f : C;
+  const float d = fmaxf((c - cs) * LOG2E, -1000.f), f = __builtin_amdgcn_exp2f(d);
+  t = wave_all_sum(f * fmaf(d, s, t));
+  s = wave_all_sum(f * s);
+  c = C;
 }
 
-// (maximum, sum, weighted sum) of two parts of a row; e^(m - M) of a part without weight is not
-// taken, and a difference that passes the float range weighs nothing
-DEV void lp_join(float& m, float& s, float& t, float m2, float s2, float t2) {
-  const float M = fmaxf(m, m2), ms = M == -INFINITY ? 0.f : M;
-  const float d = fmaxf((m - ms) * LOG2E, -200.f), d2 = fmaxf((m2 - ms) * LOG2E, -200.f);
-  const float f = __builtin_amdgcn_exp2f(d), f2 = __builtin_amdgcn_exp2f(d2);
-  t = f * fmaf(d, s, t) + f2 * fmaf(d2, s2, t2);
-  s = f * s + f2 * s2;
-  m = M;
-}
-
-// A row per workgroup.  The row is read once into registers, NV vectors a thread (a LONG row in
-// segments of that).  Every thread sums relative to its own running maximum, so the row needs one
-// exchange between waves.  Alternatives: the top-th largest of 64 partial maxima (one per lane,
-// over the waves) is a value that at least `top` elements reach; the few elements that reach it are
-// gathered in LDS and ranked there.  Where more than LP_CAND do (long ties), or too few (NaN), the
-// alternatives are found one by one, in passes over the row.
-template <typename T, int TPB, int NV, bool LONG>
-__global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void token_logprobs_kernel(
-    int V, int top, const T* __restrict__ logits, long ld, const int64_t* __restrict__ tgt, float* __restrict__ logp,
-    float* __restrict__ entropy, float* __restrict__ stats, float* __restrict__ top_logp,
-    int64_t* __restrict__ top_ids) {
-  constexpr int VEC = 16 / sizeof(T), NW = TPB / 64, SEG = TPB * NV;
-  __shared__ float part[NW][3];
+// A row per workgroup, read once: NV vectors a thread in flight, taken as they come.  A thread keeps
+// its maximum m and sums relative to a reference c, a logit that follows m when m has passed it by 5
+// or more (rare after the first vector, so no second look at the data and no rescaling as a rule):
+// with z = (x - c) log2 e, s = sum 2^z and t = sum 2^z z.  c is a logit itself, so the row of a single
+// word has s = 1 exactly.  DPP joins the lanes, LDS the waves.
+// Alternatives: the top-th largest of 64 partial maxima (one per lane, over the waves) is a value
+// that at least `top` elements reach; the few elements that reach it are gathered in LDS and ranked
+// there.  Where more than LP_CAND do (long ties), or too few (NaN), the alternatives are found one by
+// one, in passes over the row.
+template <typename T, int TPB, bool LONG>
+__global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, const T* __restrict__ logits, long ld,
+                                                             const int64_t* __restrict__ tgt, float* __restrict__ logp,
+                                                             float* __restrict__ entropy, float* __restrict__ stats,
+                                                             float* __restrict__ top_logp, int64_t* __restrict__ top_ids) {
+  constexpr int VEC = 16 / sizeof(T), NW = TPB / 64, NV = 8, SEG = TPB * NV;
+  __shared__ float part[NW][4];
   __shared__ float lane_max[NW][64];
   __shared__ uint64_t cand[LP_CAND];
-  __shared__ int ncand;
+  __shared__ int ncand, nbusy;
+  __shared__ uint16_t busy[TPB];
   const long row = blockIdx.x;
   const T* x = logits + row * ld;
   const Row<T> r(x, V);
   const int tid = threadIdx.x, w = tid >> 6, lane = tid & 63;
   const long k = tgt ? tgt[row] : -1;
   const bool hit = k >= 0 && k < V;
-  float xt = 0.f;
-  if (tid == 0) ncand = 0;
+  if (tid == 0) ncand = nbusy = 0;
   constexpr uint32_t NONE = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;
+  float m = -INFINITY, c = -INFINITY, s = 0.f, t = 0.f;
   uint4 u[NV];
-  float m = -INFINITY, s = 0.f, t = 0.f;
+#pragma unroll
+  for (int j = 0; j < NV; ++j)  // all in flight before the first is used: under no branch, the end again where past it
+    u[j] = r.base[min(j * TPB + tid, r.nvec - 1)];
+  if (tid == 0) r.trim(u[0], 0);
   for (int q0 = 0; q0 < (LONG ? r.nvec : 1); q0 += SEG) {
     const int last = r.nvec - 1 - q0;
 #pragma unroll
-    for (int j = 0; j < NV; ++j)  // all in flight before the first is used: under no branch, the end again where past it
-      u[j] = r.base[q0 + min(j * TPB + tid, last)];
-    if (q0 == 0 && tid == 0) r.trim(u[0], 0);
-#pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (last >= j * TPB && last < (j + 1) * TPB) {
-        if (j * TPB + tid > last) u[j] = make_uint4(NONE, NONE, NONE, NONE);
-        if (j * TPB + tid == last) r.trim(u[j], q0 + last);
-      }
-    float mx = m;
-#pragma unroll
     for (int j = 0; j < NV; ++j) {
       if (last >= j * TPB) {
+        if (last < (j + 1) * TPB) {
+          if (j * TPB + tid > last) u[j] = make_uint4(NONE, NONE, NONE, NONE);
+          if (j * TPB + tid == last) r.trim(u[j], q0 + last);
+        }
         float v[VEC];
         unpack<T>(u[j], v);
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, v[e]);
-      }
-      __builtin_amdgcn_sched_barrier(0);  // one vector's floats at a time: more of them at once only spill
-    }
-    if constexpr (sizeof(T) == 2) keep_packed(u);
-    if (q0 == 0 && hit) xt = to_f(x[k]);
-    const float ms = mx == -INFINITY ? 0.f : mx;
-    if (LONG && q0 > 0) lp_join(m, s, t, mx, 0.f, 0.f);
-    m = mx;
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-      if (last >= j * TPB) {
-        float v[VEC];
-        unpack<T>(u[j], v);
+        for (int e = 0; e < VEC; ++e) m = fmaxf(m, v[e]);
+        if (m - c > 5.f) {
+          const float d = fmaxf((c - m) * LOG2E, -1000.f), f = __builtin_amdgcn_exp2f(d);
+          t = f * fmaf(d, s, t);
+          s *= f;
+          c = m;
+        }
+        const float cs = c == -INFINITY ? 0.f : c;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
-          const float z = (v[e] - ms) * LOG2E, p = __builtin_amdgcn_exp2f(z);
+          const float z = (v[e] - cs) * LOG2E, p = __builtin_amdgcn_exp2f(z);
           s += p;
           t = fmaf(p, fmaxf(z, -200.f), t);  // p is 0 long before -200: a finite factor beside it
         }
       }
-      __builtin_amdgcn_sched_barrier(0);
+      if (LONG) u[j] = r.base[min(q0 + SEG + j * TPB + tid, r.nvec - 1)];  // its place in the next segment
+      __builtin_amdgcn_sched_barrier(0);  // one vector's floats at a time: more of them at once only spill
     }
   }
+  const float xt = hit ? to_f(x[k]) : 0.f;
   lane_max[w][lane] = m;
-  float ms = m, ss = s, ts = t;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1)
-    lp_join(ms, ss, ts, __shfl_xor(ms, o, 64), __shfl_xor(ss, o, 64), __shfl_xor(ts, o, 64));
+  const float wm = wave_all_max(m);
+  lp_join_lanes(c, s, t);
   if (lane == 0) {
-    part[w][0] = ms;
-    part[w][1] = ss;
-    part[w][2] = ts;
+    part[w][0] = wm;
+    part[w][1] = c;
+    part[w][2] = s;
+    part[w][3] = t;
   }
   __syncthreads();
-  float M = part[lane % NW][0], S = part[lane % NW][1], Z = part[lane % NW][2];
-#pragma unroll
-  for (int o = 1; o < NW; o <<= 1) lp_join(M, S, Z, __shfl_xor(M, o, 64), __shfl_xor(S, o, 64), __shfl_xor(Z, o, 64));
-  // the lanes join in different orders and may differ in the last bit: lane 0's holds for all, or an
-  // alternative's value would go by the place that it got in the list
-  M = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, M)));
-  S = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, S)));
-  Z = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, Z)));
+  float C = lane < NW ? part[lane][1] : -INFINITY, S = lane < NW ? part[lane][2] : 0.f, Z = lane < NW ? part[lane][3] : 0.f;
+  const float M = wave_all_max(lane < NW ? part[lane][0] : -INFINITY);
+  lp_join_lanes(C, S, Z);
   const bool none = S == 0.f;  // every logit -inf
-  const float l2 = none ? 0.f : log2f(S), ls = l2 * LN2;
+  const float ls2 = log2f(S), l2 = none ? 0.f : fmaf(C - M, LOG2E, ls2), ls = l2 * LN2;
   if (tid == 0) {
     stats[2 * row] = M;
     stats[2 * row + 1] = l2;
-    entropy[row] = none ? 0.f : (l2 - Z / S) * LN2;
+    entropy[row] = none ? 0.f : (ls2 - Z / S) * LN2;
     if (tgt) logp[row] = !hit ? 0.f : none ? -INFINITY : (xt - M) - ls;
   }
   if (top == 0) return;
@@ -196,21 +199,30 @@ __global__ __launch_bounds__(TPB) __attribute__((amdgpu_waves_per_eu(4))) void t
     if (__popcll(__ballot(key >= (bar | 1u << b))) >= top) bar |= 1u << b;
   const float least = bar <= 0x007fu ? -INFINITY
                                      : __builtin_bit_cast(float, bar & 0x8000u ? (bar << 16) & 0x7fffffffu : ~(bar << 16));
-  // a thread with such an element goes over its part of the row again: few do, and it is in the cache
-  if (m >= least)
-    for (int q = tid; q < r.nvec; q += TPB) {
-      float v[VEC];
+  // the threads with such an element are few: their parts of the row are gone over again, a vector a
+  // thread of the whole group, out of the cache
+  if (m >= least) busy[atomicAdd(&nbusy, 1)] = (uint16_t)tid;
+  __syncthreads();
+  const int per = (r.nvec + TPB - 1) / TPB;
+  for (int i0 = tid; i0 < nbusy * per; i0 += TPB) {
+    const int q = busy[i0 / per] + i0 % per * TPB;
+    if (q < r.nvec) {
+      float v[VEC], mx = -INFINITY;
       unpack<T>(r.base[q], v);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, v[e]);
+      if (mx < least) continue;
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
         if (v[e] >= least) {
-          const int c = q * VEC + e - r.skew;
-          if (c >= 0 && c < V) {
+          const int i = q * VEC + e - r.skew;
+          if (i >= 0 && i < V) {
             const int at = atomicAdd(&ncand, 1);
-            if (at < LP_CAND) cand[at] = ((uint64_t)order_key(v[e]) << 32) | (0xffffffffu - (uint32_t)c);
+            if (at < LP_CAND) cand[at] = ((uint64_t)order_key(v[e]) << 32) | (0xffffffffu - (uint32_t)i);
           }
         }
     }
+  }
   __syncthreads();
   const int nc = ncand;
   if (nc >= top && nc <= LP_CAND) {
@@ -312,16 +324,22 @@ extern "C" int imgcap_token_logprobs(int dtype, int n, int V, int top, const voi
   IMGCAP_REQUIRE(logits && entropy && stats && (!targets || logp) && (top == 0 || (top_logp && top_ids)),
                  "imgcap_token_logprobs: NULL operand");
   hipStream_t st = (hipStream_t)stream;
-#define LP_(T, TPB, NV, LONG)                                                                             \
-  hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, NV, LONG>), dim3(n), dim3(TPB), 0, st, V, top,        \
+#define LP_(T, TPB, LONG)                                                                                 \
+  hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, LONG>), dim3(n), dim3(TPB), 0, st, V, top,            \
                      (const T*)logits, (long)ld, targets, logp, entropy, stats, top_logp, top_ids)
-#define LP_T(T)                                               \
-  do {                                                        \
-    const int vec = 16 / (int)sizeof(T), nvec = (V + 2 * vec - 2) / vec; \
-    if (nvec <= 256 * 8 && n > 512) LP_(T, 256, 8, false);    \
-    else if (nvec <= 1024 * 8) LP_(T, 1024, 8, false);        \
-    else if (nvec <= 1024 * 16) LP_(T, 1024, 16, false);      \
-    else LP_(T, 1024, 8, true);                               \
+#define LP_T(T)                                                                                           \
+  do {                                                                                                    \
+    const int vec = 16 / (int)sizeof(T), nvec = (V + 2 * vec - 2) / vec;                                  \
+    if (n > 1024) {                                                                                       \
+      if (nvec <= 256 * 8) LP_(T, 256, false);                                                            \
+      else LP_(T, 256, true);                                                                             \
+    } else if (n > 512) {                                                                                 \
+      if (nvec <= 512 * 8) LP_(T, 512, false);                                                            \
+      else LP_(T, 512, true);                                                                             \
+    } else {                                                                                              \
+      if (nvec <= 1024 * 8) LP_(T, 1024, false);                                                          \
+      else LP_(T, 1024, true);                                                                            \
+    }                                                                                                     \
   } while (0)
   if (dtype == IMGCAP_BF16) LP_T(bf16);
   else LP_T(float);
