@@ -301,68 +301,92 @@ template <int BYTES> DEV Words<BYTES> load_words(const void* p) {
   return r;
 }
 
-template <typename T, int DH> struct KvTile {  // 32 tokens of one kv head, as the wave's operands
+// 32 tokens of one kv head as a wave's operands.  Pages of 16 tokens and more: 16 tokens share a
+// page, whose id is the same for the wave (TINY: an id per token, in the lanes).  Ids are looked up a
+// step ahead; one outside the cache reads page 0, and its tokens are masked.
+template <typename T, int DH, bool TINY> struct KvTile {
   static constexpr int NS = DH * sizeof(T) / 64;   // 16-byte pieces of a key row per lane
   static constexpr int VB = DH / 16 * sizeof(T);   // bytes of a value row per lane
   uint4 k[2][NS];
   Words<VB> v[2][4];
-  bool live[2];  // the page is one of the cache's (pages of 16 tokens and more)
-};
-
-template <typename T, int DH>
-DEV void kv_load(KvTile<T, DH>& t, const imgcap_paged_attn_desc& d, const int32_t* table, int kvh, int tok, int n, int lp) {
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const T* kb = (const T*)d.k + (long)kvh * d.k_head;
-  const T* vb = (const T*)d.v + (long)kvh * d.v_head;
+  int id[2];  // page of each half (TINY: of token r of it), -1 if outside the cache
+  DEV void look_up(int (&next)[2], const imgcap_paged_attn_desc& d, const int32_t* table, int tok, int lp, int r) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int t0 = tok + 16 * h;
-    if (lp >= 4) {  // the 16 tokens share a page
-      const int id = table[min(t0, n - 1) >> lp];
-      t.live[h] = (unsigned)id < (unsigned)d.pages;
-      const long pg = t.live[h] ? id : 0, off = t0 & (d.page - 1);
-      const T* kp = kb + pg * d.k_page + (off + r) * d.k_tok + g * (16 / sizeof(T));
-      const T* vp = vb + pg * d.v_page + (off + 4 * g) * d.v_tok + r * (DH / 16);
+    for (int h = 0; h < 2; ++h) next[h] = table[min((tok + 16 * h + (TINY ? r : 0)) >> lp, d.width - 1)];
+  }
+  DEV void take(const int (&next)[2], const imgcap_paged_attn_desc& d) {
 #pragma unroll
-      for (int s = 0; s < KvTile<T, DH>::NS; ++s) t.k[h][s] = *(const uint4*)(kp + s * (64 / sizeof(T)));
+    for (int h = 0; h < 2; ++h) id[h] = (unsigned)next[h] < (unsigned)d.pages ? next[h] : -1;
+  }
+  DEV void load_k(const imgcap_paged_attn_desc& d, const T* kb, int tok, int r, int g) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) t.v[h][i] = load_words<KvTile<T, DH>::VB>(vp + i * d.v_tok);
-    } else {
-      const int tk = min(t0 + r, n - 1);
-      const int id = table[tk >> lp];
-      const int slot_page = (unsigned)id < (unsigned)d.pages ? id : -1;
-      const T* kp = kb + (long)max(slot_page, 0) * d.k_page + (tk & (d.page - 1)) * d.k_tok + g * (16 / sizeof(T));
+    for (int h = 0; h < 2; ++h) {
+      const T* kp = kb + (long)max(id[h], 0) * d.k_page + ((tok + 16 * h + r) & (d.page - 1)) * d.k_tok + g * (16 / sizeof(T));
 #pragma unroll
-      for (int s = 0; s < KvTile<T, DH>::NS; ++s) t.k[h][s] = *(const uint4*)(kp + s * (64 / sizeof(T)));
-      t.live[h] = slot_page >= 0;  // of this lane's own token r
+      for (int s = 0; s < NS; ++s) k[h][s] = *(const uint4*)(kp + s * (64 / sizeof(T)));
+    }
+  }
+  DEV void load_v(const imgcap_paged_attn_desc& d, const T* vb, int tok, int r, int g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const T* vp = vb + r * (DH / 16);
+      if (!TINY) vp += (long)max(id[h], 0) * d.v_page + ((tok + 16 * h + 4 * g) & (d.page - 1)) * d.v_tok;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int vi = __shfl(slot_page, 4 * g + i, 64), vt = min(t0 + 4 * g + i, n - 1);
-        const T* vp = vb + (long)max(vi, 0) * d.v_page + (vt & (d.page - 1)) * d.v_tok + r * (DH / 16);
-        t.v[h][i] = load_words<KvTile<T, DH>::VB>(vp);
+        const T* at = vp + i * d.v_tok;
+        if (TINY)
+          at = vp + (long)max(__shfl(id[h], 4 * g + i, 64), 0) * d.v_page + ((tok + 16 * h + 4 * g + i) & (d.page - 1)) * d.v_tok;
+        v[h][i] = load_words<VB>(at);
       }
     }
   }
+  // whether lane-group token i of half h is a live position
+  DEV bool live(int h, int i, int tok, int t1, int g) const {
+    return (TINY ? __shfl(id[h], 4 * g + i, 64) : id[h]) >= 0 && tok + 16 * h + 4 * g + i < t1;
+  }
+  DEV bool all_live(int tok, int t1) const {
+    return tok + 32 <= t1 && !__any(id[0] < 0 || id[1] < 0);
+  }
+};
+
+// over the four lane groups (lane ^ 16, lane ^ 32), on swaps of 16 and of 32 lanes: after either, a
+// lane holds its own group's value and its partner's
+template <typename F> DEV float groups_fold(float v, F f) {
+  const uint32_t a = __builtin_bit_cast(uint32_t, v);
+  const auto x = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  const uint32_t x0 = x[0], x1 = x[1];
+  v = f(__builtin_bit_cast(float, x0), __builtin_bit_cast(float, x1));
+  const uint32_t b = __builtin_bit_cast(uint32_t, v);
+  const auto y = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  const uint32_t y0 = y[0], y1 = y[1];
+  return f(__builtin_bit_cast(float, y0), __builtin_bit_cast(float, y1));
 }
 
 DEV uint32_t pack_bf16(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (bf16)b) << 16);
 }
 
-template <typename T, int DH>
+template <typename T, int DH, bool TINY>
 __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit, int gtiles,
                                                          int lp, float* ws_o, float* ws_ml) {
-  using Tile = KvTile<T, DH>;
+  using Tile = KvTile<T, DH, TINY>;
   constexpr int VPL = DH / 16, LDO = DH + 4;
   extern __shared__ float sm[];  // [waves][16][LDO] of O, then [waves][16] maxima and sums
   const int nw = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
   const int row = blockIdx.x, gt = row % gtiles, kvh = (row / gtiles) % d.Hkv, b = row / gtiles / d.Hkv;
   const int split = blockIdx.y, G = d.H / d.Hkv, heads = min(16, G - 16 * gt), h0 = kvh * G + 16 * gt;
-  const int n = min(max(d.lens[b], 0), d.max_len);
-  if (split > 0 && split * (long)chunk >= n) return;
-  const int t0 = split * chunk, t1 = min(n, t0 + chunk);
+  const int t0 = split * chunk, step = 32 * nw;
   const int32_t* table = d.table + (long)b * d.table_row;
+  int tok = t0 + 32 * w;
+  Tile t;
+  int next[2];
+  t.look_up(next, d, table, tok, lp, r);  // beside the length: entries past it are as good as any
+  const int n = min(max(d.lens[b], 0), d.max_len);
+  if (split > 0 && t0 >= n) return;
+  const int t1 = min(n, t0 + chunk);
+  const T* kb = (const T*)d.k + (long)kvh * d.k_head;
+  const T* vb = (const T*)d.v + (long)kvh * d.v_head;
   const float c = d.scale * 1.44269504088896341f;
   uint4 q[Tile::NS];
 #pragma unroll
@@ -376,91 +400,108 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
 #pragma unroll
   for (int j = 0; j < VPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
-  for (int tok = t0 + 32 * w; tok < t1; tok += 32 * nw) {
-    Tile t;
-    kv_load<T, DH>(t, d, table, kvh, tok, n, lp);
-    float p[2][4];
-    float mx = -INFINITY;
+  if (tok < t1) {
+    t.take(next, d);
+    t.load_k(d, kb, tok, r, g);
+    t.load_v(d, vb, tok, r, g);
+    t.look_up(next, d, table, tok + step, lp, r);
+    while (true) {
+      const bool full = t.all_live(tok, t1), more = tok + step < t1;
+      float p[2][4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      f32x4 s4 = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int h = 0; h < 2; ++h) {
+        f32x4 s4 = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int s = 0; s < Tile::NS; ++s) {
-        if constexpr (sizeof(T) == 2) {
-          s4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[h][s]),
-                                                       __builtin_bit_cast(bf16x8, q[s]), s4, 0, 0, 0);
-        } else {
-          const f32x4 kk = __builtin_bit_cast(f32x4, t.k[h][s]), qq = __builtin_bit_cast(f32x4, q[s]);
+        for (int s = 0; s < Tile::NS; ++s) {
+          if constexpr (sizeof(T) == 2) {
+            s4 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, t.k[h][s]),
+                                                         __builtin_bit_cast(bf16x8, q[s]), s4, 0, 0, 0);
+          } else {
+            const f32x4 kk = __builtin_bit_cast(f32x4, t.k[h][s]), qq = __builtin_bit_cast(f32x4, q[s]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qq[e], s4, 0, 0, 0);
+            for (int e = 0; e < 4; ++e) s4 = __builtin_amdgcn_mfma_f32_16x16x4f32(kk[e], qq[e], s4, 0, 0, 0);
+          }
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[h][i] = s4[i] * c;
       }
+      if (!full) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const bool here = lp >= 4 ? t.live[h] : __shfl((int)t.live[h], 4 * g + i, 64);
-        const bool ok = here && tok + 16 * h + 4 * g + i < t1;
-        p[h][i] = ok ? s4[i] * c : -INFINITY;
-        mx = fmaxf(mx, p[h][i]);
-        if (!ok) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int e = 0; e < Tile::VB / 4; ++e) t.v[h][i].w[e] = 0u;
-        }
+          for (int i = 0; i < 4; ++i)
+            if (!t.live(h, i, tok, t1, g)) {
+              p[h][i] = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < Tile::VB / 4; ++e) t.v[h][i].w[e] = 0u;
+            }
       }
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), ms = mn == -INFINITY ? 0.f : mn;
-    const float alpha = __builtin_amdgcn_exp2f(m - ms);
-    m = mn;
-    l *= alpha;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p[h][i] = __builtin_amdgcn_exp2f(p[h][i] - ms);
-        l += p[h][i];
+      // the keys' registers are free: the next step's go out now, its values' after the product below
+      if (more) {
+        t.take(next, d);
+        t.load_k(d, kb, tok + step, r, g);
       }
+      float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
+                       fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
+      mx = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); });
+      if (__any(mx > m)) {  // seldom after the first steps of a long row
+        const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+        m = mn;
+        l *= alpha;
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) acc[j] *= alpha;
-    if constexpr (sizeof(T) == 2) {
-      // the weights go in as their top bf16 bits and the remainder in bf16: 15 bits and more of them,
-      // so the output carries little but its own rounding.  Both pieces are kept positive (the
-      // remainder at least 1e-30, nothing beside a weight that counts): an infinite value times a
-      // zero or negative remainder would turn the infinity into NaN.
-      uint32_t hi[4], lo[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float a = p[e >> 1][2 * (e & 1)], bb = p[e >> 1][2 * (e & 1) + 1];
-        hi[e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, bb), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-        lo[e] = pack_bf16(fmaxf(a - __builtin_bit_cast(float, hi[e] << 16), 1e-30f),
-                          fmaxf(bb - __builtin_bit_cast(float, hi[e] & 0xffff0000u), 1e-30f));
+        for (int j = 0; j < VPL; ++j) acc[j] *= alpha;
       }
-      const bf16x8 ph = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-      const bf16x8 pl = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
-        uint32_t x[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] = __builtin_amdgcn_perm(t.v[e >> 1][2 * (e & 1) + 1].w[j >> 1], t.v[e >> 1][2 * (e & 1)].w[j >> 1], sel);
-        const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph, acc[j], 0, 0, 0);
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl, acc[j], 0, 0, 0);
-      }
-    } else {
+      const float ms = m == -INFINITY ? 0.f : m;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+          p[h][i] = __builtin_amdgcn_exp2f(p[h][i] - ms);
+          l += p[h][i];
+        }
+      if constexpr (sizeof(T) == 2) {
+        // the weights go in as their top bf16 bits and the remainder in bf16: 15 bits and more of them,
+        // so the output carries little but its own rounding.  Both pieces are kept positive (the
+        // remainder at least 1e-30, nothing beside a weight that counts): an infinite value times a
+        // zero or negative remainder would turn the infinity into NaN.
+        uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int j = 0; j < VPL; ++j)
-            acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[h][i].w[j]), p[h][i], acc[j], 0,
-                                                          0, 0);
+        for (int e = 0; e < 4; ++e) {
+          const float a = p[e >> 1][2 * (e & 1)], bb = p[e >> 1][2 * (e & 1) + 1];
+          hi[e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, bb), __builtin_bit_cast(uint32_t, a), 0x07060302u);
+          lo[e] = pack_bf16(fmaxf(a - __builtin_bit_cast(float, hi[e] << 16), 1e-30f),
+                            fmaxf(bb - __builtin_bit_cast(float, hi[e] & 0xffff0000u), 1e-30f));
+        }
+        const bf16x8 ph = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+        const bf16x8 pl = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) {
+          const uint32_t sel = (j & 1) ? 0x07060302u : 0x05040100u;
+          uint32_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[e] = __builtin_amdgcn_perm(t.v[e >> 1][2 * (e & 1) + 1].w[j >> 1], t.v[e >> 1][2 * (e & 1)].w[j >> 1], sel);
+          const bf16x8 vf = __builtin_bit_cast(bf16x8, make_uint4(x[0], x[1], x[2], x[3]));
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, ph, acc[j], 0, 0, 0);
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl, acc[j], 0, 0, 0);
+        }
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int j = 0; j < VPL; ++j)
+              acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, t.v[h][i].w[j]), p[h][i], acc[j],
+                                                            0, 0, 0);
+      }
+      if (!more) break;
+      tok += step;
+      t.load_v(d, vb, tok, r, g);
+      t.look_up(next, d, table, tok + step, lp, r);
     }
   }
-  l += __shfl_xor(l, 16, 64);
-  l += __shfl_xor(l, 32, 64);
+  l = groups_fold(l, [](float x, float y) { return x + y; });
   // the waves' parts, joined in LDS: lane (r, g) holds head r, columns VPL * (4g + i) + j
   float* so = sm + (w * 16 + r) * LDO;
   float* sml = sm + nw * 16 * LDO;
@@ -499,47 +540,54 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
   }
 }
 
-// joins the chunks of a row: out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s
-template <typename T, int DH>
+// joins the chunks of a row: out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  A workgroup takes COLS
+// columns of one (request, head): all of them where there are rows enough to fill the chip, 32 where
+// there are few (a single long request of 16 heads over 391 chunks: 15.6 us by whole rows, one
+// workgroup a head).  The chunks' factors are worked out once, in LDS.
+constexpr int MAX_SPLIT = 1024;
+template <typename T, int DH, int COLS>
 __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit,
                                                          const float* __restrict__ ws_o, const float* __restrict__ ws_ml) {
-  constexpr int C4 = DH / 4, PARTS = 256 / C4;
-  __shared__ float red[4];
-  __shared__ float part[PARTS][DH + 1];
-  const int b = blockIdx.x / d.H, h = blockIdx.x % d.H;
+  constexpr int C4 = COLS / 4, PARTS = 256 / C4;
+  __shared__ float red[8];
+  __shared__ float factor[MAX_SPLIT];
+  __shared__ f32x4 part[PARTS][C4];
+  const int row = blockIdx.x / (DH / COLS), c0 = blockIdx.x % (DH / COLS) * COLS, b = row / d.H, h = row % d.H;
   const int n = min(max(d.lens[b], 0), d.max_len);
   if (n <= chunk) return;
-  const int ns = (n + chunk - 1) / chunk;
-  const float* ml = ws_ml + (long)blockIdx.x * nsplit * 2;
-  const float* oo = ws_o + (long)blockIdx.x * nsplit * DH;
-  float M = -INFINITY;
+  const int ns = (n + chunk - 1) / chunk, w = threadIdx.x >> 6;
+  const float* ml = ws_ml + (long)row * nsplit * 2;
+  float M = -INFINITY, L = 0.f;
   for (int s = threadIdx.x; s < ns; s += 256) M = fmaxf(M, ml[2 * s]);
   M = wave_max(M);
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+  if ((threadIdx.x & 63) == 0) red[w] = M;
   __syncthreads();
   M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
   const float ms = M == -INFINITY ? 0.f : M;
-  const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
-  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
-  float L = 0.f;
-  for (int s = pt; s < ns; s += PARTS) {
+  for (int s = threadIdx.x; s < ns; s += 256) {
     const float f = __builtin_amdgcn_exp2f(ml[2 * s] - ms);
+    factor[s] = f;
     L += f * ml[2 * s + 1];
-    o += f * *(const f32x4*)(oo + (long)s * DH + 4 * c4);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) part[pt][4 * c4 + i] = o[i];
-  if (c4 == 0) part[pt][DH] = L;
+  L = wave_sum(L);
+  if ((threadIdx.x & 63) == 0) red[4 + w] = L;
   __syncthreads();
-  if (threadIdx.x < DH) {
-    float v = 0.f, S = 0.f;
+  L = (red[4] + red[5]) + (red[6] + red[7]);
+  const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
+  const float* oo = ws_o + (long)row * nsplit * DH + c0 + 4 * c4;
+  f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = pt; s < ns; s += PARTS) o += factor[s] * *(const f32x4*)(oo + (long)s * DH);
+  part[pt][c4] = o;
+  __syncthreads();
+  if (threadIdx.x < COLS) {
+    const float* p = (const float*)part + threadIdx.x;
+    float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < PARTS; ++i) {
-      v += part[i][threadIdx.x];
-      S += part[i][DH];
-    }
-    ((T*)d.o)[(long)b * d.o_row + (long)h * d.o_head + threadIdx.x] = from_f<T>(S == 0.f ? 0.f : v / S);
-    if (d.lse && threadIdx.x == 0) d.lse[blockIdx.x] = S == 0.f ? -INFINITY : (M + log2f(S)) * 0.69314718055994531f;
+    for (int i = 0; i < PARTS; ++i) v += p[i * COLS];
+    const int col = c0 + threadIdx.x;
+    ((T*)d.o)[(long)b * d.o_row + (long)h * d.o_head + col] = from_f<T>(L == 0.f ? 0.f : v / L);
+    if (d.lse && col == 0) d.lse[row] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
   }
 }
 
@@ -554,8 +602,8 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
                  "paged attention: query heads must be a multiple of the key/value heads");
   IMGCAP_REQUIRE(is_pow2(d->page) && d->page <= 1024, "paged attention: page must be a power of two, at most 1024");
   IMGCAP_REQUIRE(d->pages > 0 && d->width > 0 && d->max_len > 0, "paged attention: empty cache, table or max_len");
-  IMGCAP_REQUIRE((int64_t)d->width * d->page < (1ll << 31) && d->max_len <= (int64_t)d->width * d->page,
-                 "paged attention: max_len must be within the table's width, and that below 2^31 tokens");
+  IMGCAP_REQUIRE((int64_t)d->width * d->page <= (1ll << 31) - 65536 && d->max_len <= (int64_t)d->width * d->page,
+                 "paged attention: max_len must be within the table's width, and that at most 2^31 - 65536 tokens");
   IMGCAP_REQUIRE(d->q && d->k && d->v && d->o && d->table && d->lens, "paged attention: NULL operand");
   const int64_t vec = d->dtype == IMGCAP_F32 ? 4 : 8;
   IMGCAP_REQUIRE(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && d->q_row % vec == 0 && d->q_head % vec == 0 &&
@@ -565,18 +613,22 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
   return 0;
 }
 
-// How the length is cut: workgroups of up to 4 waves, each wave 32 tokens a step
+// How the length is cut: workgroups of up to 4 waves, each wave 32 tokens a step.  A chunk is as long
+// as leaves 2048 workgroups (8 a CU, for requests of uneven lengths: 48 of up to 20011 tokens 425 us
+// with 1024, 394 with 2048 or 4096), but 512 tokens where that is less, or what leaves 256
+// workgroups where even that is less.
 struct AttnPlan { int gtiles, waves, chunk, nsplit; };
 static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
   AttnPlan p;
   p.gtiles = (d->H / d->Hkv + 15) / 16;
   p.waves = d->max_len <= 32 ? 1 : d->max_len <= 64 ? 2 : 4;
-  const int64_t rows = (int64_t)d->B * d->Hkv * p.gtiles;
-  const int64_t most = (d->max_len + 255) / 256;
-  int64_t want = rows > 0 ? (1024 + rows - 1) / rows : 1;
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  p.chunk = (int)(((d->max_len + want - 1) / want + 127) / 128 * 128);
+  const int64_t tokens = (int64_t)d->B * d->Hkv * p.gtiles * d->max_len;
+  int64_t chunk = tokens / 256 < 512 ? tokens / 256 : 512;
+  if (chunk < tokens / 2048) chunk = tokens / 2048;
+  if (chunk < (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT + 63) chunk = (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT + 63;
+  chunk = (chunk + 64) / 128 * 128;
+  if (chunk < 128) chunk = 128;
+  p.chunk = chunk > d->max_len ? (d->max_len + 127) / 128 * 128 : (int)chunk;
   p.nsplit = (d->max_len + p.chunk - 1) / p.chunk;
   return p;
 }
@@ -589,11 +641,21 @@ static void attn_launch(const imgcap_paged_attn_desc* d, const AttnPlan& p, hipS
   float* ws_o = (float*)d->ws;
   float* ws_ml = ws_o ? ws_o + (int64_t)d->B * d->H * p.nsplit * DH : nullptr;
   const int lds = (p.waves * 16 * (DH + 4) + 2 * p.waves * 16) * 4;
-  hipLaunchKernelGGL((paged_attn_kernel<T, DH>), dim3(d->B * d->Hkv * p.gtiles, p.nsplit), dim3(64 * p.waves), lds, st,
-                     *d, p.chunk, p.nsplit, p.gtiles, log2_of(d->page), ws_o, ws_ml);
-  if (p.nsplit > 1)
-    hipLaunchKernelGGL((paged_join_kernel<T, DH>), dim3(d->B * d->H), dim3(256), 0, st, *d, p.chunk, p.nsplit, ws_o,
-                       ws_ml);
+  const dim3 grid(d->B * d->Hkv * p.gtiles, p.nsplit), block(64 * p.waves);
+  if (d->page >= 16)
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, false>), grid, block, lds, st, *d, p.chunk, p.nsplit, p.gtiles,
+                       log2_of(d->page), ws_o, ws_ml);
+  else
+    hipLaunchKernelGGL((paged_attn_kernel<T, DH, true>), grid, block, lds, st, *d, p.chunk, p.nsplit, p.gtiles,
+                       log2_of(d->page), ws_o, ws_ml);
+  if (p.nsplit > 1) {
+    const int rows = d->B * d->H;
+    if (rows >= 256)
+      hipLaunchKernelGGL((paged_join_kernel<T, DH, DH>), dim3(rows), dim3(256), 0, st, *d, p.chunk, p.nsplit, ws_o, ws_ml);
+    else
+      hipLaunchKernelGGL((paged_join_kernel<T, DH, 32>), dim3(rows * (DH / 32)), dim3(256), 0, st, *d, p.chunk, p.nsplit,
+                         ws_o, ws_ml);
+  }
 }
 
 }  // namespace imgcap
