@@ -301,23 +301,47 @@ template <int BYTES> DEV Words<BYTES> load_words(const void* p) {
   return r;
 }
 
-// 32 tokens of one kv head as a wave's operands.  Pages of 16 tokens and more: 16 tokens share a
-// page, whose id is the same for the wave (TINY: an id per token, in the lanes).  Ids are looked up a
-// step ahead; one outside the cache reads page 0, and its tokens are masked.
+// The pages of a wave's steps (32 tokens each), looked up a step before their use; -1 for an id outside
+// the cache.  Pages of 16 tokens and more: 16 tokens share a page, lanes 0 and 1 hold those of the two
+// halves.  TINY: a lane holds the page of its own token r of either half.
+template <bool TINY> struct Pages {
+  static constexpr int N = TINY ? 2 : 1;
+  const int32_t* table;
+  int now[N], then[N];
+  int lp, last, pages;
+  DEV void look(int (&to)[N], int tok) const {
+    const int lane = threadIdx.x & 63, own = TINY ? lane & 15 : 16 * (lane & 1);
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = table[min((tok + 16 * i + own) >> lp, last)];
+  }
+  // nothing here waits for the request's length: entries past it are as good as any
+  DEV Pages(const imgcap_paged_attn_desc& d, const int32_t* row, int tok, int step, int lp_)
+      : table(row), lp(lp_), last(d.width - 1), pages(d.pages) {
+    look(now, tok);
+    look(then, tok + step);
+  }
+  // the pages of the step at tok, if there is one; steps are taken in order.  No branch: a load under
+  // one would be waited for, and all before it, where the paths meet.
+  DEV void take(int (&id)[2], int tok, int step, bool more) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = TINY ? now[h % N] : __builtin_amdgcn_readlane(now[0], h);
+      id[h] = !more ? id[h] : (unsigned)e < (unsigned)pages ? e : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) now[i] = then[i];
+    look(then, tok + 2 * step);
+  }
+};
+
+// 32 tokens of one kv head as a wave's operands.  A page outside the cache reads page 0, and its
+// tokens are masked.
 template <typename T, int DH, bool TINY> struct KvTile {
   static constexpr int NS = DH * sizeof(T) / 64;   // 16-byte pieces of a key row per lane
   static constexpr int VB = DH / 16 * sizeof(T);   // bytes of a value row per lane
   uint4 k[2][NS];
   Words<VB> v[2][4];
   int id[2];  // page of each half (TINY: of token r of it), -1 if outside the cache
-  DEV void look_up(int (&next)[2], const imgcap_paged_attn_desc& d, const int32_t* table, int tok, int lp, int r) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) next[h] = table[min((tok + 16 * h + (TINY ? r : 0)) >> lp, d.width - 1)];
-  }
-  DEV void take(const int (&next)[2], const imgcap_paged_attn_desc& d) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) id[h] = (unsigned)next[h] < (unsigned)d.pages ? next[h] : -1;
-  }
   DEV void load_k(const imgcap_paged_attn_desc& d, const T* kb, int tok, int r, int g) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -366,23 +390,32 @@ DEV uint32_t pack_bf16(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (bf16)b) << 16);
 }
 
-template <typename T, int DH, bool TINY>
-__global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit, int gtiles,
-                                                         int lp, float* ws_o, float* ws_ml) {
+// JOIN: the workgroup's waves share a chunk (blockIdx.x the row, blockIdx.y the chunk), 32 tokens each
+// in turn, and put their parts together in LDS.  Else each wave has a row and chunk to itself, the
+// waves of a group consecutive rows (kv heads of the same tokens, which lie side by side in memory),
+// and nothing is exchanged.  Bound by HBM where the caches are large, and more waves than two a SIMD
+// only lengthen the queues there (first scores of a wave after 16 us at 12 waves a CU): 48 requests of
+// up to 20011 tokens 393 us at two, 401 at three.
+constexpr int JOIN_WAVES = 4, MAX_SPLIT = 1024;
+template <typename T, int DH, bool TINY, bool JOIN>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
+    imgcap_paged_attn_desc d, int chunk, int nsplit, int gtiles, int lp, float* ws_o, float* ws_ml) {
   using Tile = KvTile<T, DH, TINY>;
   constexpr int VPL = DH / 16, LDO = DH + 4;
-  extern __shared__ float sm[];  // [waves][16][LDO] of O, then [waves][16] maxima and sums
-  const int nw = blockDim.x >> 6, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, g = lane >> 4;
-  const int row = blockIdx.x, gt = row % gtiles, kvh = (row / gtiles) % d.Hkv, b = row / gtiles / d.Hkv;
+  const int row = JOIN ? blockIdx.x : blockIdx.x * (blockDim.x >> 6) + w;
+  if (!JOIN && row >= d.B * d.Hkv * gtiles) return;
+  const int gt = row % gtiles, kvh = (row / gtiles) % d.Hkv, b = row / gtiles / d.Hkv;
   const int split = blockIdx.y, G = d.H / d.Hkv, heads = min(16, G - 16 * gt), h0 = kvh * G + 16 * gt;
-  const int t0 = split * chunk, step = 32 * nw;
+  const int t0 = split * chunk, step = JOIN ? 32 * JOIN_WAVES : 32;
   const int32_t* table = d.table + (long)b * d.table_row;
-  int tok = t0 + 32 * w;
+  int tok = t0 + (JOIN ? 32 * w : 0);
   Tile t;
-  int next[2];
-  t.look_up(next, d, table, tok, lp, r);  // beside the length: entries past it are as good as any
-  const int n = min(max(d.lens[b], 0), d.max_len);
+  Pages<TINY> pages(d, table, tok, step, lp);
+  int len = __builtin_amdgcn_readfirstlane(d.lens[b]);
+  asm volatile("" : "+v"(pages.now[0]), "+s"(len));  // loaded side by side, not one after the other
+  const int n = min(max(len, 0), d.max_len);
   if (split > 0 && t0 >= n) return;
   const int t1 = min(n, t0 + chunk);
   const T* kb = (const T*)d.k + (long)kvh * d.k_head;
@@ -401,10 +434,9 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
   for (int j = 0; j < VPL; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, l = 0.f;
   if (tok < t1) {
-    t.take(next, d);
+    pages.take(t.id, tok, step, true);
     t.load_k(d, kb, tok, r, g);
     t.load_v(d, vb, tok, r, g);
-    t.look_up(next, d, table, tok + step, lp, r);
     while (true) {
       const bool full = t.all_live(tok, t1), more = tok + step < t1;
       float p[2][4];
@@ -437,10 +469,10 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
             }
       }
       // the keys' registers are free: the next step's go out now, its values' after the product below
-      if (more) {
-        t.take(next, d);
-        t.load_k(d, kb, tok + step, r, g);
-      }
+      // (after the last step this one's again, from the cache)
+      pages.take(t.id, tok + step, step, more);
+      const int ahead = more ? tok + step : tok;
+      t.load_k(d, kb, ahead, r, g);
       float mx = fmaxf(fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[0][2], p[0][3])),
                        fmaxf(fmaxf(p[1][0], p[1][1]), fmaxf(p[1][2], p[1][3])));
       mx = groups_fold(mx, [](float x, float y) { return fmaxf(x, y); });
@@ -498,44 +530,83 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
       if (!more) break;
       tok += step;
       t.load_v(d, vb, tok, r, g);
-      t.look_up(next, d, table, tok + step, lp, r);
     }
   }
   l = groups_fold(l, [](float x, float y) { return x + y; });
-  // the waves' parts, joined in LDS: lane (r, g) holds head r, columns VPL * (4g + i) + j
-  float* so = sm + (w * 16 + r) * LDO;
-  float* sml = sm + nw * 16 * LDO;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) so[VPL * (4 * g + i) + j] = acc[j][i];
-  if (g == 0) {
-    sml[w * 16 + r] = m;
-    sml[(nw + w) * 16 + r] = l;
-  }
-  __syncthreads();
   const bool whole = n <= chunk;
-  for (int e = threadIdx.x; e < heads * DH; e += blockDim.x) {
-    const int hd = e / DH, col = e % DH;
-    float M = -INFINITY;
-    for (int i = 0; i < nw; ++i) M = fmaxf(M, sml[i * 16 + hd]);
-    const float ms = M == -INFINITY ? 0.f : M;
-    float L = 0.f, o = 0.f;
-    for (int i = 0; i < nw; ++i) {
-      const float f = __builtin_amdgcn_exp2f(sml[i * 16 + hd] - ms);
-      L += f * sml[(nw + i) * 16 + hd];
-      o += f * sm[(i * 16 + hd) * LDO + col];
-    }
-    const long bh = (long)b * d.H + h0 + hd;
+  // lane (r, g) holds head r, columns VPL * (4 g + i) + j: DH / 4 consecutive ones
+  if constexpr (!JOIN) {
+    if (r >= heads) return;
+    const long bh = (long)b * d.H + h0 + r;
     if (whole) {
-      ((T*)d.o)[(long)b * d.o_row + (long)(h0 + hd) * d.o_head + col] = from_f<T>(L == 0.f ? 0.f : o / L);
-      if (d.lse && col == 0) d.lse[bh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
+      const float f = l == 0.f ? 0.f : 1.f / l;
+      T* o = (T*)d.o + (long)b * d.o_row + (long)(h0 + r) * d.o_head + VPL * 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) o[VPL * i + j] = from_f<T>(l == 0.f ? 0.f : acc[j][i] * f);
+      if (d.lse && g == 0) d.lse[bh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
     } else {
-      ws_o[(bh * nsplit + split) * DH + col] = o;
-      if (col == 0) {
-        ws_ml[(bh * nsplit + split) * 2] = M;
-        ws_ml[(bh * nsplit + split) * 2 + 1] = L;
+      float* o = ws_o + (bh * nsplit + split) * DH + VPL * 4 * g;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VPL; j += 4)
+          *(f32x4*)(o + VPL * i + j) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+      if (g == 0) *(f32x2*)(ws_ml + (bh * nsplit + split) * 2) = f32x2{m, l};
+    }
+  } else {
+    __shared__ float ml[JOIN_WAVES][2][16];
+    __shared__ float sm[JOIN_WAVES / 2 * 16 * LDO];  // parts, to the common maximum
+    if (g == 0) {
+      ml[w][0][r] = m;
+      ml[w][1][r] = l;
+    }
+    __syncthreads();
+    float M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int i = 0; i < JOIN_WAVES; ++i) M = fmaxf(M, ml[i][0][r]);
+    const float ms = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int i = 0; i < JOIN_WAVES; ++i) L += __builtin_amdgcn_exp2f(ml[i][0][r] - ms) * ml[i][1][r];
+    const float f = __builtin_amdgcn_exp2f(m - ms) * (!whole ? 1.f : L == 0.f ? 0.f : 1.f / L);
+    // half of the waves hand their parts to the other half, lane to lane, so that four parts lie in LDS
+    constexpr int HALF = JOIN_WAVES / 2;
+    float* so = sm + (w % HALF * 16 + r) * LDO + VPL * 4 * g;
+    if (w >= HALF) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VPL; j += 4)
+          *(f32x4*)(so + VPL * i + j) = f * f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    }
+    __syncthreads();
+    if (w < HALF) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < VPL; j += 4)
+          *(f32x4*)(so + VPL * i + j) += f * f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < heads * (DH / 4); e += 64 * JOIN_WAVES) {
+      const int hd = e / (DH / 4), col = 4 * (e % (DH / 4));
+      const long bh = (long)b * d.H + h0 + hd;
+      f32x4 o = *(const f32x4*)(sm + hd * LDO + col);
+#pragma unroll
+      for (int i = 1; i < HALF; ++i) o += *(const f32x4*)(sm + (i * 16 + hd) * LDO + col);
+      if (whole) {
+        T* out = (T*)d.o + (long)b * d.o_row + (long)(h0 + hd) * d.o_head + col;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) out[i] = from_f<T>(o[i]);
+      } else {
+        *(f32x4*)(ws_o + (bh * nsplit + split) * DH + col) = o;
       }
+    }
+    if (w == 0 && g == 0 && r < heads) {
+      const long bh = (long)b * d.H + h0 + r;
+      if (!whole) *(f32x2*)(ws_ml + (bh * nsplit + split) * 2) = f32x2{M, L};
+      else if (d.lse) d.lse[bh] = L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994531f;
     }
   }
 }
@@ -544,7 +615,6 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(imgcap_paged_attn_desc 
 // columns of one (request, head): all of them where there are rows enough to fill the chip, 32 where
 // there are few (a single long request of 16 heads over 391 chunks: 15.6 us by whole rows, one
 // workgroup a head).  The chunks' factors are worked out once, in LDS.
-constexpr int MAX_SPLIT = 1024;
 template <typename T, int DH, int COLS>
 __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit,
                                                          const float* __restrict__ ws_o, const float* __restrict__ ws_ml) {
@@ -613,22 +683,29 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
   return 0;
 }
 
-// How the length is cut: workgroups of up to 4 waves, each wave 32 tokens a step.  A chunk is as long
-// as leaves 2048 workgroups (8 a CU, for requests of uneven lengths: 48 of up to 20011 tokens 425 us
-// with 1024, 394 with 2048 or 4096), but 512 tokens where that is less, or what leaves 256
-// workgroups where even that is less.
-struct AttnPlan { int gtiles, waves, chunk, nsplit; };
+// How the length is cut (times of bf16 unless said, MI355X, calls replayed from a graph).
+//  - Up to 64 tokens, two steps, a wave has the row to itself: 512 rows of up to 52 tokens 4.5 us
+//    against 4.9 by workgroups of 4 waves; fp32, whose step is longer, up to 32 (40 rows of 49 tokens
+//    5.5 by workgroups, 6.5 by waves).
+//  - Longer ones go to workgroups of 4 waves (8: 32 requests of up to 2048 tokens with 8 kv heads 44 us,
+//    4: 40, a wave each: 51), whole up to 512 tokens, up to 1024 where the rows alone are a
+//    workgroup to each CU: the second launch that joins parts costs 4 us (512 rows of up to 600
+//    tokens 12.2 whole, 15.9 in chunks of 512).
+//  - Else chunks of 512 tokens, shorter (to 128) where that leaves CUs without one, longer where it
+//    leaves more than 4096 (48 requests of up to 20011 tokens, 8 kv heads of 128: 402 us with 2048
+//    workgroups, 393 with 4096; 432 with 1024).
+struct AttnPlan { int gtiles, chunk, nsplit; bool join; };
 static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
   AttnPlan p;
   p.gtiles = (d->H / d->Hkv + 15) / 16;
-  p.waves = d->max_len <= 32 ? 1 : d->max_len <= 64 ? 2 : 4;
-  const int64_t tokens = (int64_t)d->B * d->Hkv * p.gtiles * d->max_len;
+  p.join = d->max_len > (d->dtype == IMGCAP_F32 ? 32 : 64);
+  const int64_t rows = (int64_t)d->B * d->Hkv * p.gtiles, tokens = rows * d->max_len;
   int64_t chunk = tokens / 256 < 512 ? tokens / 256 : 512;
-  if (chunk < tokens / 2048) chunk = tokens / 2048;
-  if (chunk < (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT + 63) chunk = (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT + 63;
-  chunk = (chunk + 64) / 128 * 128;
+  if (chunk < tokens / 4096) chunk = tokens / 4096;
   if (chunk < 128) chunk = 128;
-  p.chunk = chunk > d->max_len ? (d->max_len + 127) / 128 * 128 : (int)chunk;
+  if (chunk < (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT) chunk = (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT;
+  if (chunk > d->max_len || d->max_len <= (rows >= 256 ? 1024 : 512)) chunk = d->max_len;
+  p.chunk = (int)((chunk + 31) / 32 * 32);
   p.nsplit = (d->max_len + p.chunk - 1) / p.chunk;
   return p;
 }
@@ -640,14 +717,21 @@ template <typename T, int DH>
 static void attn_launch(const imgcap_paged_attn_desc* d, const AttnPlan& p, hipStream_t st) {
   float* ws_o = (float*)d->ws;
   float* ws_ml = ws_o ? ws_o + (int64_t)d->B * d->H * p.nsplit * DH : nullptr;
-  const int lds = (p.waves * 16 * (DH + 4) + 2 * p.waves * 16) * 4;
-  const dim3 grid(d->B * d->Hkv * p.gtiles, p.nsplit), block(64 * p.waves);
-  if (d->page >= 16)
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, false>), grid, block, lds, st, *d, p.chunk, p.nsplit, p.gtiles,
-                       log2_of(d->page), ws_o, ws_ml);
-  else
-    hipLaunchKernelGGL((paged_attn_kernel<T, DH, true>), grid, block, lds, st, *d, p.chunk, p.nsplit, p.gtiles,
-                       log2_of(d->page), ws_o, ws_ml);
+  const int rows_kv = d->B * d->Hkv * p.gtiles, lp = log2_of(d->page);
+  // few rows: a wave to a workgroup, so that they spread over the CUs
+  const int waves = rows_kv * (int64_t)p.nsplit >= 1024 ? 4 : 1;
+#define PA_(TINY, JOIN)                                                                                          \
+  hipLaunchKernelGGL((paged_attn_kernel<T, DH, TINY, JOIN>),                                                     \
+                     dim3(JOIN ? rows_kv : (rows_kv + waves - 1) / waves, p.nsplit),                             \
+                     dim3(64 * (JOIN ? JOIN_WAVES : waves)), 0, st, *d, p.chunk, p.nsplit, p.gtiles, lp, ws_o, ws_ml)
+  if (d->page >= 16) {
+    if (p.join) PA_(false, true);
+    else PA_(false, false);
+  } else {
+    if (p.join) PA_(true, true);
+    else PA_(true, false);
+  }
+#undef PA_
   if (p.nsplit > 1) {
     const int rows = d->B * d->H;
     if (rows >= 256)
