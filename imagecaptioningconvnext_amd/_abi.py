@@ -54,6 +54,18 @@ class MhaDesc(ctypes.Structure):
         ("probs", c_void_p)]
 
 
+class PagedPlanDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("B", "width", "page", "pool", "tokens")] + [("table_row", c_int64)] + [
+        (n, c_void_p) for n in ("past", "add", "table", "free_ids", "count", "count_out", "lens", "starts", "slots",
+                                "rows", "positions", "waits", "ws")]
+
+
+class LogprobDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "n", "V", "top")] + [("ld", c_int64), ("ldd", c_int64)] + [
+        (n, c_void_p) for n in ("logits", "targets", "logp", "entropy", "stats", "top_logp", "top_ids", "dlogp",
+                                "dentropy", "dlogits")]
+
+
 class PagedWriteDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int32) for n in ("dtype", "n", "heads", "dh", "page", "pages")] + [
         (n, c_int64) for n in ("k_row", "k_head", "v_row", "v_head", "kc_page", "kc_tok", "kc_head", "vc_page",
@@ -154,12 +166,12 @@ _SIGS = {
                              c_void_p],
     "imgcap_greedy_select": [c_int, c_int, c_int, c_void_p, c_int64, c_int, c_int, c_int64, c_void_p, c_void_p,
                              c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p],
-    "imgcap_paged_plan": [c_int] * 5 + [c_void_p] * 3 + [c_int64] + [c_void_p] * 11,
+    "imgcap_paged_plan": [ctypes.POINTER(PagedPlanDesc), c_void_p],
     "imgcap_paged_write": [ctypes.POINTER(PagedWriteDesc), c_void_p],
     "imgcap_paged_attention_ws": [ctypes.POINTER(PagedAttnDesc), ctypes.POINTER(c_int64)],
     "imgcap_paged_attention": [ctypes.POINTER(PagedAttnDesc), c_void_p],
-    "imgcap_token_logprobs": [c_int] * 4 + [c_void_p, c_int64] + [c_void_p] * 7,
-    "imgcap_token_logprobs_bwd": [c_int] * 3 + [c_void_p, c_int64] + [c_void_p] * 6 + [c_int64, c_void_p],
+    "imgcap_token_logprobs": [ctypes.POINTER(LogprobDesc), c_void_p],
+    "imgcap_token_logprobs_bwd": [ctypes.POINTER(LogprobDesc), c_void_p],
     "imgcap_slice_reduce": [c_int64, c_int, c_void_p, c_int64, c_float, c_int64, c_void_p, c_void_p, c_void_p],
 }
 

@@ -333,19 +333,26 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(int V, int bloc
 
 using namespace imgcap;
 
-extern "C" int imgcap_token_logprobs(int dtype, int n, int V, int top, const void* logits, int64_t ld,
-                                     const int64_t* targets, float* logp, float* entropy, float* stats,
-                                     float* top_logp, int64_t* top_ids, void* stream) {
-  IMGCAP_REQUIRE(dtype == IMGCAP_F32 || dtype == IMGCAP_BF16, "imgcap_token_logprobs: dtype must be fp32 or bf16");
-  IMGCAP_REQUIRE(n >= 0 && V > 0 && ld >= V, "imgcap_token_logprobs: bad n / V / ld");
+static int lp_check(const imgcap_logprob_desc* d, const char* name) {
+  const std::string at = std::string(name) + ": ";
+  IMGCAP_REQUIRE(d != nullptr, at + "desc NULL");
+  IMGCAP_REQUIRE(d->dtype == IMGCAP_F32 || d->dtype == IMGCAP_BF16, at + "dtype must be fp32 or bf16");
+  IMGCAP_REQUIRE(d->n >= 0 && d->V > 0 && (d->n <= 1 || d->ld >= d->V), at + "bad n / V / ld");
+  return 0;
+}
+
+extern "C" int imgcap_token_logprobs(const imgcap_logprob_desc* d, void* stream) {
+  if (int rc = lp_check(d, "imgcap_token_logprobs")) return rc;
+  const int n = d->n, V = d->V, top = d->top;
   IMGCAP_REQUIRE(top >= 0 && top <= LP_MAX_TOP && top <= V, "imgcap_token_logprobs: top must be 0 .. min(64, V)");
   if (n == 0) return 0;
-  IMGCAP_REQUIRE(logits && entropy && stats && (!targets || logp) && (top == 0 || (top_logp && top_ids)),
+  IMGCAP_REQUIRE(d->logits && d->entropy && d->stats && (!d->targets || d->logp) &&
+                     (top == 0 || (d->top_logp && d->top_ids)),
                  "imgcap_token_logprobs: NULL operand");
   hipStream_t st = (hipStream_t)stream;
 #define LP_(T, TPB, LONG)                                                                                 \
   hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, LONG>), dim3(n), dim3(TPB), 0, st, V, top,            \
-                     (const T*)logits, (long)ld, targets, logp, entropy, stats, top_logp, top_ids)
+                     (const T*)d->logits, (long)d->ld, d->targets, d->logp, d->entropy, d->stats, d->top_logp, d->top_ids)
 #define LP_T(T)                                                                                           \
   do {                                                                                                    \
     const int vec = 16 / (int)sizeof(T), nvec = (V + 2 * vec - 2) / vec;                                  \
@@ -359,7 +366,7 @@ extern "C" int imgcap_token_logprobs(int dtype, int n, int V, int top, const voi
       else LP_(T, 1024, true);                                                                            \
     }                                                                                                     \
   } while (0)
-  if (dtype == IMGCAP_BF16) LP_T(bf16);
+  if (d->dtype == IMGCAP_BF16) LP_T(bf16);
   else LP_T(float);
 #undef LP_T
 #undef LP_
@@ -367,26 +374,25 @@ extern "C" int imgcap_token_logprobs(int dtype, int n, int V, int top, const voi
   return 0;
 }
 
-extern "C" int imgcap_token_logprobs_bwd(int dtype, int n, int V, const void* logits, int64_t ld,
-                                         const int64_t* targets, const float* stats, const float* entropy,
-                                         const float* dlogp, const float* dentropy, void* dlogits, int64_t ldd,
-                                         void* stream) {
-  IMGCAP_REQUIRE(dtype == IMGCAP_F32 || dtype == IMGCAP_BF16, "imgcap_token_logprobs_bwd: dtype must be fp32 or bf16");
-  IMGCAP_REQUIRE(n >= 0 && V > 0 && ld >= V && ldd >= V, "imgcap_token_logprobs_bwd: bad n / V / ld / ldd");
+extern "C" int imgcap_token_logprobs_bwd(const imgcap_logprob_desc* d, void* stream) {
+  if (int rc = lp_check(d, "imgcap_token_logprobs_bwd")) return rc;
+  const int n = d->n, V = d->V;
+  IMGCAP_REQUIRE(n <= 1 || d->ldd >= V, "imgcap_token_logprobs_bwd: bad ldd");
   if (n == 0) return 0;
-  IMGCAP_REQUIRE(logits && stats && entropy && dlogits && (!dlogp || targets),
+  IMGCAP_REQUIRE(d->logits && d->stats && d->entropy && d->dlogits && (!d->dlogp || d->targets),
                  "imgcap_token_logprobs_bwd: NULL operand");
-  IMGCAP_REQUIRE(logits != dlogits || ld == ldd || n == 1, "imgcap_token_logprobs_bwd: in place needs equal pitches");
+  IMGCAP_REQUIRE(d->logits != d->dlogits || d->ld == d->ldd || n == 1,
+                 "imgcap_token_logprobs_bwd: in place needs equal pitches");
   hipStream_t st = (hipStream_t)stream;
 #define LPB_(T)                                                                                                     \
   do {                                                                                                              \
     const int vec = 16 / (int)sizeof(T), blocks = ((V + 2 * vec - 2) / vec + 1023) / 1024;                          \
     IMGCAP_REQUIRE((int64_t)n * blocks < (1ll << 31), "imgcap_token_logprobs_bwd: too many rows");                  \
     hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3((unsigned)n * blocks), dim3(256), 0, st, V, blocks,       \
-                       (const T*)logits, (long)ld, targets, stats, entropy, dlogp, dentropy, (T*)dlogits, (long)ldd,  \
+                       (const T*)d->logits, (long)d->ld, d->targets, d->stats, d->entropy, d->dlogp, d->dentropy, (T*)d->dlogits, (long)d->ldd, \
                        (int64_t)n * V * (int64_t)sizeof(T) > (128ll << 20) ? 1 : 0);                                \
   } while (0)
-  if (dtype == IMGCAP_BF16) LPB_(bf16);
+  if (d->dtype == IMGCAP_BF16) LPB_(bf16);
   else LPB_(float);
 #undef LPB_
   IMGCAP_CHECK_LAUNCH("imgcap_token_logprobs_bwd");

@@ -11,29 +11,14 @@ namespace imgcap {
 // Integer prefix sums give each request its place on the stack of free pages and its first token;
 // every token then finds its request by bisection of the starts.  A step of up to PLAN_ROWS requests
 // is one pass of one workgroup with 32-bit sums in the lanes; up to PLAN_TOKENS tokens it also lays
-// out the tokens itself, from LDS.  It is latency that counts there: lengths, count and the page that
-// a request has open are loaded at once, one more dependent load follows (the page taken off the
-// stack).  More tokens go to a second launch over the whole chip; more requests (or sums that might
+// out the tokens itself, from LDS.  It is latency that counts there, so loads come in two rounds: the
+// lengths and the stack's height; then the pages that requests have open, the top of the stack and the
+// pages of ended requests, all of which the tokens find in LDS.  Barriers wait for LDS alone, not for
+// the global stores and loads on their way.  More tokens go to a second launch over the whole chip; more requests (or sums that might
 // pass 32 bits) to a pass in chunks with 64-bit sums.
-constexpr int PLAN_ROWS = 1024, PLAN_TOKENS = 4096, PLAN_CAP = 1 << 20;
+constexpr int PLAN_ROWS = 1024, PLAN_TOKENS = 4096, PLAN_CAP = 1 << 20, PLAN_BACK = 2048;
 
-struct PlanArgs {
-  int B, width, lp, pool, tokens;
-  const int32_t* past;
-  const int32_t* add;
-  int32_t* table;
-  long table_row;
-  int32_t* free_ids;
-  const int32_t* count;
-  int32_t* count_out;
-  int32_t* lens;
-  int32_t* starts;
-  int64_t* slots;
-  int32_t* rows;
-  int64_t* positions;
-  int32_t* waits;
-  int32_t* ws;  // [B] first page of each request on the stack, [B] = the stack's top
-};
+struct PlanArgs : imgcap_paged_plan_desc { int lp; };  // lp: log2 of the page size
 
 DEV int wave_scan_incl(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8: within 16 lanes
@@ -53,17 +38,13 @@ DEV long wave_scan_incl(long v) {
   return v;
 }
 // inclusive prefix over the block; `total` gets the block's sum.  red: blockDim / 64 values.
-template <typename I> DEV I block_scan_incl(I v, I* red, I& total) {
+DEV long block_scan_incl(long v, long* red, long& total) {
   const int w = threadIdx.x >> 6, nw = blockDim.x >> 6;
   v = wave_scan_incl(v);
-  if (nw == 1) {
-    total = __shfl(v, 63, 64);
-    return v;
-  }
   __syncthreads();
   if ((threadIdx.x & 63) == 63) red[w] = v;
   __syncthreads();
-  I before = 0, all = 0;
+  long before = 0, all = 0;
   for (int i = 0; i < nw; ++i) {
     if (i < w) before += red[i];
     all += red[i];
@@ -71,8 +52,37 @@ template <typename I> DEV I block_scan_incl(I v, I* red, I& total) {
   total = all;
   return v + before;
 }
+// a barrier of what lies in LDS
+DEV void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+// inclusive prefixes of two values over the block and their sums; red: 16 pairs
+DEV void block_scan2(int& a, int& b, int2* red, int& sum_a, int& sum_b) {
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63, nw = blockDim.x >> 6;
+  a = wave_scan_incl(a);
+  b = wave_scan_incl(b);
+  if (nw == 1) {
+    sum_a = __builtin_amdgcn_readlane(a, 63);
+    sum_b = __builtin_amdgcn_readlane(b, 63);
+    return;
+  }
+  lds_barrier();
+  if (lane == 63) red[w] = make_int2(a, b);
+  lds_barrier();
+  const int2 mine = lane < nw ? red[lane] : make_int2(0, 0);
+  const int ia = wave_scan_incl(mine.x), ib = wave_scan_incl(mine.y);
+  sum_a = __builtin_amdgcn_readlane(ia, 63);
+  sum_b = __builtin_amdgcn_readlane(ib, 63);
+  const int uw = __builtin_amdgcn_readfirstlane(w);
+  if (uw > 0) {
+    a += __builtin_amdgcn_readlane(ia, uw - 1);
+    b += __builtin_amdgcn_readlane(ib, uw - 1);
+  }
+}
 
-// the request of token i: starts[r] <= i < starts[r + 1] (n requests)
+// the request of token i: starts[r] <= i < starts[r + 1] (n requests; the last of those that start alike)
 DEV int plan_row(const int32_t* starts, int n, int i) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
@@ -93,50 +103,53 @@ DEV void plan_none(const PlanArgs& a, int i) {
   a.rows[i] = -1;
   a.positions[i] = 0;
 }
-// the id of page pi of a request that holds `have` pages and takes the next ones from place `at` of
-// the stack down; the token that opens a page enters it into the table
-DEV int plan_page(const PlanArgs& a, int row, int pi, int have, int at, long pos) {
-  const int id = a.free_ids[at - (pi - have)];
+// the token that opens a page enters it into the table
+DEV void plan_enter(const PlanArgs& a, int row, int pi, long pos, int id) {
   if (((int)pos & ((1 << a.lp) - 1)) == 0) a.table[(long)row * a.table_row + pi] = id;
-  return id;
 }
 
 __global__ __launch_bounds__(PLAN_ROWS) void paged_plan_kernel(PlanArgs a, int expand) {
-  __shared__ int red[16];
-  __shared__ int starts_s[PLAN_ROWS + 1], at_s[PLAN_ROWS], past_s[PLAN_ROWS], open_s[PLAN_ROWS];
+  __shared__ int2 red[16];
+  __shared__ int starts_s[PLAN_ROWS], at_s[PLAN_ROWS], past_s[PLAN_ROWS], open_s[PLAN_ROWS];
+  __shared__ int before_s[PLAN_ROWS], stack_s[PLAN_ROWS], push_s[PLAN_BACK];
+  // the arguments in one go: the compiler would fetch each where it is first used, one wait after another
+  asm volatile("" ::"s"(a.B), "s"(a.past), "s"(a.add), "s"(a.count), "s"(a.table), "s"(a.free_ids), "s"(a.lp), "s"(a.pool),
+               "s"(a.width), "s"(a.tokens));
   const int T = blockDim.x, b = threadIdx.x, page = 1 << a.lp;
   const bool in = b < a.B;
   const int past = in ? a.past[b] : 0, add = in ? a.add[b] : -1;
-  int top = min(max(*a.count, 0), a.pool);
+  const int height = min(max(*a.count, 0), a.pool);
   const long lp = past, la = add, room = (long)a.width << a.lp;
   const bool live = add >= 0;
   const int have = (int)((max(lp, 0l) + page - 1) >> a.lp);
-  int open = -1;  // the page that the request's next token goes to, if it has one open
+  int open = -1, under = -1;  // the page that the request's next token goes to; the b-th page from the stack's top
   if (live && past > 0 && (past & (page - 1)) && (past >> a.lp) < a.width) open = a.table[b * a.table_row + (past >> a.lp)];
+  if (expand && b < height) under = a.free_ids[height - 1 - b];
   const int back = in && !live ? min(have, a.width) : 0;
   bool fits = live && past >= 0 && lp + la <= room;
   const int asked = fits ? min(add, a.tokens + 1) : 0;  // one past the capacity is as far as it counts
-  int asked_all, need_all, back_all = 0;
-  const int tok = block_scan_incl(asked, red, asked_all);
+  int tok = asked, given = back, asked_all, back_all, need_all, none;
+  block_scan2(tok, given, red, asked_all, back_all);
   fits = fits && tok <= a.tokens;
   const int need = fits ? (int)((lp + la + page - 1) >> a.lp) - have : 0;
-  const int upto = block_scan_incl(need, red, need_all);
-  if (__syncthreads_or(back > 0)) {  // pages of ended requests go back on the stack, in the requests' order
-    const int before = block_scan_incl(back, red, back_all) - back;
-    starts_s[b] = back;
-    at_s[b] = before;
-    __syncthreads();
-    for (int r = b >> 6; r < a.B; r += T >> 6)
-      for (int j = b & 63; j < starts_s[r]; j += 64)
-        if ((long)top + at_s[r] + j < a.pool) a.free_ids[top + at_s[r] + j] = a.table[r * a.table_row + j];
-    __syncthreads();
-    top = (int)min((long)top + back_all, (long)a.pool);
+  int upto = need, zero = 0;
+  block_scan2(upto, zero, red, need_all, none);
+  const int top = (int)min((long)height + back_all, (long)a.pool);
+  if (back_all > 0) {  // pages of ended requests go back on the stack, in the requests' order
+    before_s[b] = given - back;
+    lds_barrier();
+    for (int at = b; at < back_all; at += T) {
+      const int r = plan_row(before_s, a.B, at), id = a.table[r * a.table_row + (at - before_s[r])];
+      if ((long)height + at < a.pool) a.free_ids[height + at] = id;
+      if (at < PLAN_BACK) push_s[at] = id;
+    }
   }
   const bool granted = fits && (need == 0 || upto <= top);
   int start = tok - asked, total = asked_all, used = need_all;
   if (asked_all > a.tokens || need_all > top) {  // some request waits: what the others get, again
-    start = block_scan_incl(granted ? add : 0, red, total) - (granted ? add : 0);
-    block_scan_incl(granted ? need : 0, red, used);
+    int got = granted ? add : 0, took = granted ? need : 0;
+    block_scan2(got, took, red, total, used);
+    start = got - (granted ? add : 0);
   }
   if (in) {
     a.lens[b] = live ? past + (granted ? add : 0) : 0;
@@ -156,7 +169,9 @@ __global__ __launch_bounds__(PLAN_ROWS) void paged_plan_kernel(PlanArgs a, int e
   at_s[b] = top - 1 - (upto - need);
   past_s[b] = past;
   open_s[b] = open;
-  __syncthreads();
+  stack_s[b] = under;
+  if (back_all > PLAN_BACK) __syncthreads();  // some of the pages put back are read from the stack
+  else lds_barrier();
   for (int i = b; i < a.tokens; i += T) {
     if (i >= total) {
       plan_none(a, i);
@@ -165,7 +180,13 @@ __global__ __launch_bounds__(PLAN_ROWS) void paged_plan_kernel(PlanArgs a, int e
     const int r = plan_row(starts_s, a.B, i), p0 = past_s[r];
     const long pos = (long)p0 + (i - starts_s[r]);
     const int pi = (int)(pos >> a.lp), h = (int)(((long)p0 + page - 1) >> a.lp);
-    plan_put(a, i, r, pos, pi < h ? open_s[r] : plan_page(a, r, pi, h, at_s[r], pos));
+    int id = open_s[r];
+    if (pi >= h) {  // a page of the stack: place `at`, counted from its bottom
+      const int at = at_s[r] - (pi - h), pushed = at - height, deep = height - 1 - at;
+      id = pushed >= 0 && pushed < PLAN_BACK ? push_s[pushed] : deep >= 0 && deep < T ? stack_s[deep] : a.free_ids[at];
+      plan_enter(a, r, pi, pos, id);
+    }
+    plan_put(a, i, r, pos, id);
   }
 }
 
@@ -229,29 +250,68 @@ __global__ __launch_bounds__(1024) void paged_plan_long_kernel(PlanArgs a) {
   }
 }
 
-// lays out the tokens after either planner: SLOT_TOKENS a workgroup, the starts in LDS if they fit
+// lays out the tokens after either planner: four consecutive ones a thread (one search for them, 16-byte
+// stores where the outputs are so aligned), the starts in LDS if they fit.  Bound by latency and the
+// 20 bytes a token that it writes.  A request's old length is its new one less its tokens (past itself may
+// be the array that the new ones went to).
 constexpr int SLOT_TOKENS = 1024, SLOT_ROWS = 4096;
-__global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a) {
+__global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a, int aligned) {
   __shared__ int32_t starts_s[SLOT_ROWS];
+  asm volatile("" ::"s"(a.B), "s"(a.lens), "s"(a.starts), "s"(a.ws), "s"(a.table), "s"(a.free_ids), "s"(a.lp), "s"(a.pool),
+               "s"(a.slots), "s"(a.rows), "s"(a.positions), "s"(a.tokens));  // in one go
   const int32_t* starts = a.starts;
+  const int total = a.starts[a.B], top = a.ws[a.B], page = 1 << a.lp;
+  const long i0 = (long)blockIdx.x * SLOT_TOKENS + 4 * threadIdx.x;
   if (a.B <= SLOT_ROWS) {
     for (int i = threadIdx.x; i < a.B; i += 256) starts_s[i] = a.starts[i];
     __syncthreads();
     starts = starts_s;
   }
-  const int total = a.starts[a.B], top = a.ws[a.B], page = 1 << a.lp;
+  if (i0 >= a.tokens) return;
+  int r = plan_row(starts, a.B, (int)min(i0, (long)total)), begin = starts[r];
+  int end = r + 1 < a.B ? starts[r + 1] : total, p0 = a.lens[r] - (end - begin), at = top - 1 - a.ws[r], known = -1, id = -1;
+  int64_t slot[4], position[4];
+  int32_t row[4];
 #pragma unroll
-  for (int j = 0; j < SLOT_TOKENS / 256; ++j) {
-    const long i = (long)blockIdx.x * SLOT_TOKENS + 256 * j + threadIdx.x;
-    if (i >= a.tokens) break;
-    if (i >= total) {
-      plan_none(a, (int)i);
-      continue;
+  for (int j = 0; j < 4; ++j) {
+    const long i = i0 + j;
+    slot[j] = -1;
+    position[j] = 0;
+    row[j] = -1;
+    if (i >= total || i >= a.tokens) continue;
+    if (i >= end) {  // the next request that has a token here
+      do {
+        begin = end;
+        ++r;
+        end = r + 1 < a.B ? starts[r + 1] : total;
+      } while (i >= end);
+      p0 = a.lens[r] - (end - begin);
+      at = top - 1 - a.ws[r];
+      known = -1;
     }
-    const int r = plan_row(starts, a.B, (int)i), p0 = a.past[r];
-    const long pos = (long)p0 + (i - starts[r]);
-    const int pi = (int)(pos >> a.lp), h = (int)(((long)p0 + page - 1) >> a.lp);
-    plan_put(a, (int)i, r, pos, pi < h ? a.table[r * a.table_row + pi] : plan_page(a, r, pi, h, top - 1 - a.ws[r], pos));
+    const long pos = (long)p0 + (i - begin);
+    const int pi = (int)(pos >> a.lp), h = (int)(((long)p0 + page - 1) >> a.lp), off = (int)pos & (page - 1);
+    if (pi != known) id = pi < h ? a.table[(long)r * a.table_row + pi] : a.free_ids[at - (pi - h)];
+    known = pi;
+    if (pi >= h && off == 0) a.table[(long)r * a.table_row + pi] = id;
+    slot[j] = (unsigned)id < (unsigned)a.pool ? ((int64_t)id << a.lp) + off : -1;
+    position[j] = pos;
+    row[j] = r;
+  }
+  if (aligned && i0 + 4 <= a.tokens) {
+    *(longlong2*)(a.slots + i0) = make_longlong2(slot[0], slot[1]);
+    *(longlong2*)(a.slots + i0 + 2) = make_longlong2(slot[2], slot[3]);
+    *(longlong2*)(a.positions + i0) = make_longlong2(position[0], position[1]);
+    *(longlong2*)(a.positions + i0 + 2) = make_longlong2(position[2], position[3]);
+    *(int4*)(a.rows + i0) = make_int4(row[0], row[1], row[2], row[3]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j < a.tokens) {
+        a.slots[i0 + j] = slot[j];
+        a.positions[i0 + j] = position[j];
+        a.rows[i0 + j] = row[j];
+      }
   }
 }
 
@@ -746,23 +806,23 @@ static void attn_launch(const imgcap_paged_attn_desc* d, const AttnPlan& p, hipS
 
 using namespace imgcap;
 
-extern "C" int imgcap_paged_plan(int B, int width, int page, int pool, int tokens, const int32_t* past,
-                                 const int32_t* add, int32_t* table, int64_t table_row, int32_t* free_ids,
-                                 const int32_t* count, int32_t* count_out, int32_t* lens, int32_t* starts,
-                                 int64_t* slots, int32_t* rows, int64_t* positions, int32_t* waits, int32_t* ws,
-                                 void* stream) {
-  IMGCAP_REQUIRE(B > 0 && width > 0 && pool > 0 && tokens >= 0, "imgcap_paged_plan: B, width and pool must be positive");
-  IMGCAP_REQUIRE(is_pow2(page) && page <= 1024, "imgcap_paged_plan: page must be a power of two, at most 1024");
-  IMGCAP_REQUIRE((int64_t)width * page < (1ll << 31), "imgcap_paged_plan: width * page must be below 2^31");
-  IMGCAP_REQUIRE(table_row >= width, "imgcap_paged_plan: table rows overlap");
-  IMGCAP_REQUIRE(past && add && table && free_ids && count && count_out && lens && starts && waits &&
-                     (tokens == 0 || (slots && rows && positions)),
+extern "C" int imgcap_paged_plan(const imgcap_paged_plan_desc* d, void* stream) {
+  IMGCAP_REQUIRE(d != nullptr, "imgcap_paged_plan: desc NULL");
+  const int B = d->B, width = d->width, tokens = d->tokens;
+  IMGCAP_REQUIRE(B > 0 && width > 0 && d->pool > 0 && tokens >= 0,
+                 "imgcap_paged_plan: B, width and pool must be positive, tokens not negative");
+  IMGCAP_REQUIRE(is_pow2(d->page) && d->page <= 1024, "imgcap_paged_plan: page must be a power of two, at most 1024");
+  IMGCAP_REQUIRE((int64_t)width * d->page < (1ll << 31), "imgcap_paged_plan: width * page must be below 2^31");
+  IMGCAP_REQUIRE(d->table_row >= width, "imgcap_paged_plan: table rows overlap");
+  IMGCAP_REQUIRE(d->past && d->add && d->table && d->free_ids && d->count && d->count_out && d->lens && d->starts &&
+                     d->waits && (tokens == 0 || (d->slots && d->rows && d->positions)),
                  "imgcap_paged_plan: NULL operand");
-  const PlanArgs a{B, width, log2_of(page), pool, tokens, past, add, table, (long)table_row, free_ids, count, count_out,
-                   lens, starts, slots, rows, positions, waits, ws};
+  PlanArgs a;
+  (imgcap_paged_plan_desc&)a = *d;
+  a.lp = log2_of(d->page);
   const bool fast = B <= PLAN_ROWS && tokens <= PLAN_CAP && width <= PLAN_CAP;
   const bool one = fast && tokens <= PLAN_TOKENS;
-  IMGCAP_REQUIRE(one || ws, "imgcap_paged_plan: NULL workspace");
+  IMGCAP_REQUIRE(one || d->ws, "imgcap_paged_plan: NULL workspace");
   hipStream_t st = (hipStream_t)stream;
   if (fast) {
     const int most = one && tokens > B ? (tokens < PLAN_ROWS ? tokens : PLAN_ROWS) : B;
@@ -772,7 +832,7 @@ extern "C" int imgcap_paged_plan(int B, int width, int page, int pool, int token
   }
   if (!one && tokens > 0)
     hipLaunchKernelGGL(paged_slots_kernel, dim3((unsigned)(((int64_t)tokens + SLOT_TOKENS - 1) / SLOT_TOKENS)), dim3(256),
-                       0, st, a);
+                       0, st, a, aligned16(d->slots) && aligned16(d->rows) && aligned16(d->positions) ? 1 : 0);
   IMGCAP_CHECK_LAUNCH("imgcap_paged_plan");
   return 0;
 }

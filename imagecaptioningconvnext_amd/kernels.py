@@ -621,33 +621,32 @@ def transpose(x, out=None):
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _one_device(name, *ts):
-    """Index of the GPU that all of ``ts`` (None left out) live on."""
-    dev = ts[0].get_device()
-    if dev < 0:
-        raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
+def _one_device(name, t0, *ts):
+    """Index of the GPU that all of the tensors (None left out) live on."""
+    dev = t0.get_device()
     for t in ts:
         if t is not None and t.get_device() != dev:
-            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
+            raise ValueError(f"{name}: tensors on {t0.device} and {t.device}")
+    if dev < 0:
+        raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
     return dev
 
 
-def _call_on(dev, name, *args):
+def _run_on(dev, name, desc):
     """Return code of ``name`` on the current stream of GPU ``dev``, whichever is the current one."""
     fn = getattr(_abi.lib(), name)
     if dev == torch.cuda.current_device():
-        return fn(*args, _raw_stream(dev))
+        return fn(desc, _raw_stream(dev))
     with torch.cuda.device(dev):
-        return fn(*args, _raw_stream(dev))
+        return fn(desc, _raw_stream(dev))
 
 
-def _want(name, what, t, dtype, shape, contiguous=True):
-    if t.dtype != dtype:
+def _want(name, what, t, dtype, shape):
+    """``t`` is a contiguous tensor of ``dtype`` and ``shape``, or a TypeError / ValueError."""
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: {what} must be {dtype}, got {t.dtype}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: {what} must have shape {shape}, got {tuple(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"{name}: {what} must be contiguous")
+    if t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: {what} must be contiguous of shape {shape}, got {tuple(t.shape)}")
 
 
 def _int_rows(name, what, t, rows):
@@ -670,7 +669,8 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     left goes to ``count_out`` (default: count itself).  ``tokens`` is the step's capacity, at least
     the sum of new.  Returns (lens [B] int32, starts [B + 1] int32, slots [tokens] int64, rows
     [tokens] int32, positions [tokens] int64, waits [B] int32); pass it back as ``out`` to have it
-    filled again (a captured graph's outputs).  A request that does not fit -- lengths past the table,
+    filled again (a captured graph's outputs); ``past`` may be its lens, so that a loop's lengths go on
+    in place.  A request that does not fit -- lengths past the table,
     no page left, no token left -- waits: waits[b] = 1, nothing else of it changes."""
     name = "paged_plan"
     count_out = count if count_out is None else count_out
@@ -699,9 +699,11 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
         _want(name, "positions", positions, i64, (tokens,))
         _want(name, "waits", waits, i32, (B,))
     ws = None if B <= _PLAN_ROWS and tokens <= _PLAN_TOKENS and width <= _PLAN_CAP else past.new_empty(B + 1)
-    rc = _call_on(dev, "imgcap_paged_plan", B, width, page, free.numel(), tokens, past.data_ptr(), new.data_ptr(),
-                  table.data_ptr(), table_row, free.data_ptr(), count.data_ptr(), count_out.data_ptr(), lens.data_ptr(),
-                  starts.data_ptr(), slots.data_ptr(), rows.data_ptr(), positions.data_ptr(), waits.data_ptr(), ptr(ws))
+    d = _abi.PagedPlanDesc(B, width, page, free.numel(), tokens, table_row, past.data_ptr(), new.data_ptr(),
+                           table.data_ptr(), free.data_ptr(), count.data_ptr(), count_out.data_ptr(), lens.data_ptr(),
+                           starts.data_ptr(), slots.data_ptr(), rows.data_ptr(), positions.data_ptr(),
+                           waits.data_ptr(), ptr(ws))
+    rc = _run_on(dev, "imgcap_paged_plan", d)
     if rc:
         _abi.fail("imgcap_paged_plan", rc)
     return out
@@ -737,7 +739,7 @@ def paged_write(k, v, k_cache, v_cache, slots):
     d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0],
                             vc[1], vc[2], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                             slots.data_ptr())
-    rc = _call_on(dev, "imgcap_paged_write", d)
+    rc = _run_on(dev, "imgcap_paged_write", d)
     if rc:
         _abi.fail("imgcap_paged_write", rc)
 
@@ -762,7 +764,8 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
     if out is None:
         out = q.new_empty((B, H, dh))
     else:
-        _want(name, "out", out, q.dtype, (B, H, dh), contiguous=False)
+        if out.dtype is not q.dtype or out.shape != q.shape:
+            raise ValueError(f"paged_attention: out must be {q.dtype} of shape {tuple(q.shape)}")
     qs, os_ = q.stride(), out.stride()
     if qs[2] != 1 or os_[2] != 1:
         raise ValueError("paged_attention: q and out must have unit inner stride")
@@ -774,13 +777,13 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
                            dh ** -0.5 if scale is None else scale, qs[0], qs[1], os_[0], os_[1], ks[0], ks[1], ks[2],
                            vs[0], vs[1], vs[2], table_row, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                            out.data_ptr(), ptr(lse), table.data_ptr(), lens.data_ptr(), None, 0)
-    rc = _call_on(dev, "imgcap_paged_attention", d)
+    rc = _run_on(dev, "imgcap_paged_attention", d)
     if rc == _abi.IMGCAP_EWORKSPACE:  # a split length: the parts' maxima, sums and outputs; nothing ran yet
         need = ctypes.c_int64(0)
         _abi.check("imgcap_paged_attention_ws", d, need)
         ws = q.new_empty(need.value, dtype=torch.uint8)
         d.ws, d.ws_bytes = ws.data_ptr(), need.value
-        rc = _call_on(dev, "imgcap_paged_attention", d)
+        rc = _run_on(dev, "imgcap_paged_attention", d)
     if rc:
         _abi.fail("imgcap_paged_attention", rc)
     return out
@@ -815,8 +818,9 @@ def token_logprobs(logits, targets=None, V=None, *, top=0):
         logp = logits.new_empty(n, dtype=f32)
     entropy, stats = logits.new_empty(n, dtype=f32), logits.new_empty((n, 2), dtype=f32)
     top_logp, top_ids = logits.new_empty((n, top), dtype=f32), logits.new_empty((n, top), dtype=torch.int64)
-    rc = _call_on(dev, "imgcap_token_logprobs", dt(logits), n, V, top, logits.data_ptr(), ld, ptr(targets), ptr(logp),
-                  entropy.data_ptr(), stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+    d = _abi.LogprobDesc(dt(logits), n, V, top, ld, 0, logits.data_ptr(), ptr(targets), ptr(logp), entropy.data_ptr(),
+                         stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
+    rc = _run_on(dev, "imgcap_token_logprobs", d)
     if rc:
         _abi.fail("imgcap_token_logprobs", rc)
     return logp, entropy, stats, top_logp, top_ids
@@ -852,8 +856,9 @@ def token_logprobs_bwd(logits, targets, stats, entropy, dlogp=None, dentropy=Non
         m, cols, pitch = _logit_rows(name, dlogits, None)
         if m != n or cols < V:
             raise ValueError(f"token_logprobs_bwd: dlogits must be [{n}, >= {V}]")
-    rc = _call_on(dev, "imgcap_token_logprobs_bwd", dt(logits), n, V, logits.data_ptr(), ld, ptr(targets),
-                  stats.data_ptr(), entropy.data_ptr(), ptr(dlogp), ptr(dentropy), dlogits.data_ptr(), pitch)
+    d = _abi.LogprobDesc(dt(logits), n, V, 0, ld, pitch, logits.data_ptr(), ptr(targets), None, entropy.data_ptr(),
+                         stats.data_ptr(), None, None, ptr(dlogp), ptr(dentropy), dlogits.data_ptr())
+    rc = _run_on(dev, "imgcap_token_logprobs_bwd", d)
     if rc:
         _abi.fail("imgcap_token_logprobs_bwd", rc)
     return dlogits

@@ -512,7 +512,8 @@ int imgcap_sort_gather_rows(int dtype, int B, int P, int E, int L, const int64_t
  * and its position p sits in slot table[b, p / page] * page + p % page.
  *
  * imgcap_paged_plan: one step's pages, slots and positions from the requests' lengths.
- *   past[B]   tokens of request b in the cache; add[B] tokens it gets now, negative: it has ended
+ *   past[B]   tokens of request b in the cache (may be lens itself); add[B] tokens it gets now,
+ *             negative: it has ended
  *   table     [B, table_row] int32; entries of the pages a request holds are read, those of the
  *             pages it gets are written (nothing else of it is)
  *   free_ids  [pool] int32: the free pages are free_ids[0 .. *count); ended requests' pages are
@@ -525,10 +526,24 @@ int imgcap_sort_gather_rows(int dtype, int B, int P, int E, int L, const int64_t
  *   token i of the step: slots[i], rows[i] its request, positions[i]; behind the last one -1, -1, 0,
  *   and slot -1 where the page's id is outside [0, pool).
  *   ws: B + 1 int32 of scratch (NULL where B <= 1024, tokens <= 4096 and width <= 2^20).  Requests must not share the pages that one of them gives back. */
-int imgcap_paged_plan(int B, int width, int page, int pool, int tokens, const int32_t* past, const int32_t* add,
-                      int32_t* table, int64_t table_row, int32_t* free_ids, const int32_t* count,
-                      int32_t* count_out, int32_t* lens, int32_t* starts, int64_t* slots, int32_t* rows,
-                      int64_t* positions, int32_t* waits, int32_t* ws, void* stream);
+typedef struct imgcap_paged_plan_desc {
+  int32_t B, width, page, pool, tokens;
+  int64_t table_row;
+  const int32_t* past;
+  const int32_t* add;
+  int32_t* table;
+  int32_t* free_ids;
+  const int32_t* count;
+  int32_t* count_out;
+  int32_t* lens;
+  int32_t* starts;
+  int64_t* slots;
+  int32_t* rows;
+  int64_t* positions;
+  int32_t* waits;
+  int32_t* ws;
+} imgcap_paged_plan_desc;
+int imgcap_paged_plan(const imgcap_paged_plan_desc* d, void* stream);
 
 /* Key and value rows k/v [n, heads, dh] (element strides *_row, *_head; unit inner stride) to their
  * slots of the two caches (element strides *_page, *_tok, *_head).  A slot outside [0, pages * page)
@@ -576,16 +591,26 @@ int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream);
  * logit rows [n, V] (pitch ld): logp[n] (0 where the target is outside [0, V); targets may be NULL),
  * entropy[n] in nats, stats[n, 2] = (maximum, log2 of the sum of e^(x - maximum)) for the backward,
  * top_logp / top_ids [n, top] in falling order, ties to the lower index, NaN last.  Logits of -inf
- * have no weight; a row of them alone gives logp -inf and entropy 0. */
-int imgcap_token_logprobs(int dtype, int n, int V, int top, const void* logits, int64_t ld, const int64_t* targets,
-                          float* logp, float* entropy, float* stats, float* top_logp, int64_t* top_ids,
-                          void* stream);
-/* Its gradient: dlogits[n, V] (pitch ldd, written; in place of the logits if the pitches agree) from
- * dlogp[n] and dentropy[n] (either may be NULL = 0); a row whose target is outside [0, V) has none
- * from dlogp.  The alternatives are not differentiated. */
-int imgcap_token_logprobs_bwd(int dtype, int n, int V, const void* logits, int64_t ld, const int64_t* targets,
-                              const float* stats, const float* entropy, const float* dlogp, const float* dentropy,
-                              void* dlogits, int64_t ldd, void* stream);
+ * have no weight; a row of them alone gives logp -inf and entropy 0.
+ * imgcap_token_logprobs_bwd: dlogits[n, V] (pitch ldd, written; in place of the logits if the pitches
+ * agree) from dlogp[n] and dentropy[n] (either may be NULL = 0) and the forward's stats and entropy; a
+ * row whose target is outside [0, V) has none from dlogp.  The alternatives are not differentiated. */
+typedef struct imgcap_logprob_desc {
+  int32_t dtype, n, V, top;
+  int64_t ld, ldd;
+  const void* logits;
+  const int64_t* targets;
+  float* logp;
+  float* entropy;
+  float* stats;
+  float* top_logp;
+  int64_t* top_ids;
+  const float* dlogp;
+  const float* dentropy;
+  void* dlogits;
+} imgcap_logprob_desc;
+int imgcap_token_logprobs(const imgcap_logprob_desc* d, void* stream);
+int imgcap_token_logprobs_bwd(const imgcap_logprob_desc* d, void* stream);
 
 /* elementwise helpers */
 int imgcap_cast(int in_dtype, int out_dtype, int64_t n, const void* x, void* y, void* stream);

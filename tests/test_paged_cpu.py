@@ -72,10 +72,6 @@ def test_write_of_nothing_is_nothing():
     assert _abi.lib().imgcap_paged_write(ctypes.byref(d), None) == 0
 
 
-_PLAN = dict(B=2, width=4, page=16, pool=8, tokens=2, past=A, add=A, table=A, table_row=4, free=A, count=A, count_out=A,
-             lens=A, starts=A, slots=A, rows=A, positions=A, waits=A, ws=A)
-
-
 @pytest.mark.parametrize("kw,why", [
     (dict(B=0), "positive"), (dict(width=0), "positive"), (dict(pool=0), "positive"), (dict(tokens=-1), "positive"),
     (dict(page=3), "power of two"), (dict(page=4096), "power of two"), (dict(width=1 << 28, table_row=1 << 28), "2^31"),
@@ -84,36 +80,46 @@ _PLAN = dict(B=2, width=4, page=16, pool=8, tokens=2, past=A, add=A, table=A, ta
     (dict(ws=None, width=(1 << 20) + 1, table_row=(1 << 20) + 1), "NULL"),
 ])
 def test_plan_refuses(kw, why):
-    assert _abi.lib().imgcap_paged_plan(*{**_PLAN, **kw}.values(), None) == -1
+    d = _abi.PagedPlanDesc(2, 4, 16, 8, 2, 4, *([A] * 13))
+    for k, v in kw.items():
+        setattr(d, k, v)
+    assert _abi.lib().imgcap_paged_plan(ctypes.byref(d), None) == -1
     assert why in _said()
+    assert _abi.lib().imgcap_paged_plan(None, None) == -1
 
 
-@pytest.mark.parametrize("args,why", [
-    ((2, 4, 100, 0, A, 100, None, None, A, A, None, None), "dtype"),
-    ((1, 4, 100, 65, A, 100, None, None, A, A, A, A), "top"), ((1, 4, 8, 9, A, 8, None, None, A, A, A, A), "top"),
-    ((1, 4, 100, -1, A, 100, None, None, A, A, A, A), "top"), ((1, 4, 0, 0, A, 100, None, None, A, A, None, None), "bad"),
-    ((1, -1, 9, 0, A, 9, None, None, A, A, None, None), "bad"), ((1, 4, 100, 0, A, 99, None, None, A, A, None, None), "bad"),
-    ((1, 4, 100, 3, A, 100, None, None, A, A, None, A), "NULL"), ((1, 4, 100, 0, A, 100, A, None, A, A, None, None), "NULL"),
+def _logprobs(**kw):
+    d = _abi.LogprobDesc(_abi.BF16, 4, 100, 3, 100, 100, *([A] * 10))
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(dtype=2), "dtype"), (dict(top=65), "top"), (dict(V=8, top=9), "top"), (dict(top=-1), "top"), (dict(V=0), "bad"),
+    (dict(n=-1), "bad"), (dict(ld=99), "bad"), (dict(top_logp=None), "NULL"), (dict(top_ids=None), "NULL"),
+    (dict(logp=None), "NULL"), (dict(stats=None), "NULL"), (dict(logits=None), "NULL"), (dict(entropy=None), "NULL"),
 ])
-def test_logprobs_refuses(args, why):
-    assert _abi.lib().imgcap_token_logprobs(*args, None) == -1
+def test_logprobs_refuses(kw, why):
+    assert _abi.lib().imgcap_token_logprobs(ctypes.byref(_logprobs(**kw)), None) == -1
     assert why in _said()
+    assert _abi.lib().imgcap_token_logprobs(None, None) == -1
 
 
-@pytest.mark.parametrize("args,why", [
-    ((2, 4, 100, A, 100, A, A, A, A, A, A, 100), "dtype"), ((1, 4, 100, A, 100, A, A, A, A, A, A, 99), "bad"),
-    ((1, 4, 100, A, 100, None, A, A, A, A, A, 100), "NULL"), ((1, 4, 100, A, 100, A, None, A, A, A, A, 100), "NULL"),
-    ((1, 4, 100, A, 100, A, A, A, A, A, A, 104), "in place"),
+@pytest.mark.parametrize("kw,why", [
+    (dict(dtype=2), "dtype"), (dict(ldd=99), "bad"), (dict(ld=99), "bad"), (dict(targets=None), "NULL"),
+    (dict(stats=None), "NULL"), (dict(entropy=None), "NULL"), (dict(dlogits=None), "NULL"), (dict(ldd=104), "in place"),
 ])
-def test_logprobs_bwd_refuses(args, why):
-    assert _abi.lib().imgcap_token_logprobs_bwd(*args, None) == -1
+def test_logprobs_bwd_refuses(kw, why):
+    assert _abi.lib().imgcap_token_logprobs_bwd(ctypes.byref(_logprobs(**kw)), None) == -1
     assert why in _said()
+    assert _abi.lib().imgcap_token_logprobs_bwd(None, None) == -1
 
 
 def test_no_rows_is_nothing():
-    L = _abi.lib()
-    assert L.imgcap_token_logprobs(1, 0, 10, 3, None, 10, None, None, None, None, None, None, None) == 0
-    assert L.imgcap_token_logprobs_bwd(0, 0, 10, None, 10, None, None, None, None, None, None, 10, None) == 0
+    d = _abi.LogprobDesc(_abi.F32, 0, 10, 3, 10, 10)
+    assert _abi.lib().imgcap_token_logprobs(ctypes.byref(d), None) == 0
+    assert _abi.lib().imgcap_token_logprobs_bwd(ctypes.byref(d), None) == 0
 
 
 def test_wrappers_refuse_cpu_tensors():

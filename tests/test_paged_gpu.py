@@ -503,3 +503,38 @@ def test_serving_steps(hip_device, page):
                 dk[b, j], dv[b, j] = x, y
         out, _, tol, _ = _reference(q, dk, dv, torch.arange(B).view(B, 1), [len(d) for d in dense], dh ** -0.5)
         assert bool(((got - out).abs() <= tol).all())
+
+
+def test_plan_in_place_lengths(hip_device):
+    """past and the returned lengths are one buffer, step after step, in both launch forms."""
+    K, dev = _k(), hip_device
+    i32 = dict(dtype=torch.int32, device=dev)
+    for B, page, add in ((20, 4, 3), (30, 16, 400), (1500, 8, 2)):
+        g = torch.Generator().manual_seed(21)
+        width, pool = 4 * (add + page) // page + 2, 0
+        pool = B * width
+        table, free = torch.full((B, width), -1, **i32), torch.randperm(pool, generator=g).to(**i32)
+        count, tokens = torch.tensor([pool], **i32), B * add + 1
+        hl, ht, hf, hc = [0] * B, table.tolist(), free.tolist(), pool
+        out = None
+        lens = torch.zeros(B, **i32)
+        for step in range(4):
+            new = torch.randint(0, add + 1, (B,), generator=g)
+            out = K.paged_plan(lens, new.to(**i32), table, free, count, page, tokens, out=out)
+            want, ht, hf, hc = _plan_ref(hl, new.tolist(), ht, hf, hc, page, tokens)
+            assert [x.tolist() for x in out] == list(want) and table.tolist() == ht and count.item() == hc
+            lens, hl = out[0], want[0]
+
+
+def test_plan_outputs_at_odd_places(hip_device):
+    """Outputs that do not start on 16 bytes, inside wider buffers that stay as they are around them."""
+    K, dev = _k(), hip_device
+    for case in (_plan_case(9, 64, 1000, 2000, 22), _plan_case(40, 16, 60, 5, 23)):
+        past, tokens = case[0], case[6]
+        B = len(past)
+        bufs = [torch.full((n + 3,), 55, dtype=d, device=dev) for n, d in zip(
+            (B, B + 1, tokens, tokens, tokens, B), (torch.int32, torch.int32, torch.int64, torch.int32, torch.int64,
+                                                    torch.int32))]
+        _plan_check(case, dev, out=tuple(b[1:-2] for b in bufs))
+        for b in bufs:
+            assert b[0] == 55 and bool((b[-2:] == 55).all())
