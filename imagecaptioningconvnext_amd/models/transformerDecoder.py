@@ -54,6 +54,25 @@ class _TransformerTF(torch.autograd.Function):
         return (None, denc, None, None, None, None) + grads
 
 
+class _TransformerLogProbs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, engine, encoder_out, caps, caplens, key_ids, pad_id, top, *params):
+        s = engine.forward(encoder_out, caps, caplens, key_ids=key_ids, pad_id=pad_id, loss=False)
+        ctx.engine, ctx.s = engine, s
+        ctx.enc_shape, ctx.enc_dtype = encoder_out.shape, encoder_out.dtype
+        logp, entropy, top_logp, top_ids = engine.logprobs(s, top)
+        ctx.mark_non_differentiable(top_logp, top_ids)
+        return logp, entropy, top_logp, top_ids
+
+    @staticmethod
+    def backward(ctx, dlogp, dentropy, _dtop, _dids):
+        eng, s = ctx.engine, ctx.s
+        gbuf = torch.empty_like(eng.fp.grad)
+        eng.logprobs_backward(s, dlogp, dentropy, gbuf=gbuf, want_denc=bool(ctx.needs_input_grad[1]))
+        denc = s["denc"].reshape(ctx.enc_shape).to(ctx.enc_dtype) if s["denc"] is not None else None
+        return (None, denc, None, None, None, None, None) + tuple(eng.fp.g(n, buf=gbuf) for n in eng.fp.params)
+
+
 class TransformerDecoder(nn.Module):
     def __init__(self, embed_dim, decoder_dim, vocab_size, maxLen, device, wordMap, pretrained_embeddings_path,
                  fine_tune_embeddings, dropout=0.5, encoder_dim=1024, num_heads=8, num_layers=6,
@@ -90,15 +109,27 @@ class TransformerDecoder(nn.Module):
             self._engine = TransformerEngine(self, dev, self.compute_dtype)
         return self._engine
 
+    @staticmethod
+    def _padding(encoded_captions, tgt_key_padding_mask):
+        """(key_ids, pad_id) of the self-attention: the mask's ones are padding (none without a mask)."""
+        if tgt_key_padding_mask is None:
+            return torch.zeros_like(encoded_captions), 1
+        return tgt_key_padding_mask.to(torch.int64).contiguous(), 1
+
+    def logProbs(self, encoder_out, encoded_captions, caption_lengths, tgt_key_padding_mask=None, top=0):
+        """Log-probabilities of the captions' own tokens, teacher forced: (logp [B, L], entropy [B, L] in
+        nats, top_logp [B, L, top], top_ids [B, L, top]); position l predicts token l + 1, positions past
+        a caption's last target have logp 0.  One pass over the logits, which are never held in fp32.
+        Differentiable in logp and entropy (scoring, policy-gradient training on sampled captions)."""
+        eng = self.engine()
+        key_ids, pad_id = self._padding(encoded_captions, tgt_key_padding_mask)
+        return _TransformerLogProbs.apply(eng, encoder_out, encoded_captions, caption_lengths, key_ids, pad_id, top,
+                                          *eng.fp.params.values())
+
     def forwardWithTeacherForcing(self, encoder_out, encoded_captions, caption_lengths, tgt_key_padding_mask):
         eng = self.engine()
         decode_lengths = (caption_lengths.squeeze(1) - 1).tolist()  # transformerDecoder.py:92
-        if tgt_key_padding_mask is None:
-            key_ids, pad_id = None, -1  # no padding mask (-1 never matches a token id)
-            key_ids = torch.zeros_like(encoded_captions)
-            pad_id = 1
-        else:
-            key_ids, pad_id = tgt_key_padding_mask.to(torch.int64).contiguous(), 1
+        key_ids, pad_id = self._padding(encoded_captions, tgt_key_padding_mask)
         preds = _TransformerTF.apply(eng, encoder_out, encoded_captions, caption_lengths, key_ids, pad_id,
                                      *eng.fp.params.values())
         return preds, encoded_captions, decode_lengths

@@ -177,6 +177,7 @@ class TransformerEngine:
             lens = lens.to(torch.int64)
         tmask, targets, metrics = K.tf_targets(caps if caps.dtype == torch.int64 else caps.to(torch.int64), lens)
         s["tmask"] = tmask
+        s["targets"] = targets
         if loss:
             logits = torch.empty(BL, self.Vpad, **ctd)
             K.gemm(x, fp.w("fc_out.weight"), trans_b=True, bias=fp.f32("fc_out.bias"), out=logits, N=V)
@@ -212,6 +213,35 @@ class TransformerEngine:
                                  drop_stream=sid, dr=dy, cb=cb)
         return ds, dy
 
+    # -- log-probabilities of the captions' own tokens (scoring, policy-gradient training) ---
+    def logprobs(self, s, top=0):
+        """Of a forward(loss=False): log-probability of every target token, entropy of every position
+        and its ``top`` best alternatives, (logp [B, L], entropy [B, L], top_logp [B, L, top], top_ids
+        [B, L, top]) in one pass over the logits (imgcap_token_logprobs).  Positions past a caption's
+        last target have logp 0; their entropy is that of the row as it stands."""
+        B, L, V = s["B"], s["L"], self.V
+        logits = torch.empty(B * L, self.Vpad, device=s["xL"].device, dtype=self.ct)
+        K.gemm(s["xL"], self.fp.w("fc_out.weight"), trans_b=True, bias=self.fp.f32("fc_out.bias"), out=logits, N=V)
+        logp, entropy, stats, top_logp, top_ids = K.token_logprobs(logits, s["targets"], V, top=top)
+        s["logprobs"] = (logits, stats, entropy)
+        return logp.view(B, L), entropy.view(B, L), top_logp.view(B, L, top), top_ids.view(B, L, top)
+
+    def logprobs_backward(self, s, dlogp=None, dentropy=None, gbuf=None, want_denc=False):
+        """Gradients of every parameter (and, ``want_denc``, of the encoder's output: s["denc"]) from
+        those of logprobs' logp and entropy [B, L] (either may be None) into ``gbuf``; positions past a
+        caption's last target have none."""
+        logits, stats, entropy = s["logprobs"]
+        V = self.V
+
+        def rows(g):
+            return None if g is None else torch.where(s["tmask"], g.float(), 0.0).reshape(-1)
+
+        dl = torch.empty_like(logits)
+        if self.Vpad > V:
+            dl[:, V:] = 0
+        K.token_logprobs_bwd(logits, s["targets"], stats, entropy, rows(dlogp), rows(dentropy), V=V, dlogits=dl)
+        return self.backward(s, dlogits=dl, gbuf=gbuf, want_denc=want_denc)
+
     def greedy(self, encoder_out, start_id, end_id, maxlen):
         """transformerDecoder.py:110-160 (forwardWithoutTeacherForcing) with a key/value cache.
 
@@ -233,13 +263,25 @@ class TransformerEngine:
         return preds, seqs
 
     # -- step-wise decoding primitives (greedy above, beam search in beam.py) ---------------
-    def decode_init(self, encoder_out, maxlen):
+    def decode_init(self, encoder_out, maxlen, paged=None):
         """Decoding state: the per-layer cross-attention K/V of the projected memory (computed
-        once, :112-114) and an empty per-layer cache of (q | k | v) rows for ``maxlen`` positions."""
+        once, :112-114) and an empty per-layer cache of (q | k | v) rows for ``maxlen`` positions.
+
+        ``paged`` (default: beyond 64 positions, which the tile of the dense cache's attention kernel
+        holds): keys and values lie in a pool of token-sized pages instead (kernels.paged_plan /
+        paged_write / paged_attention), for any number of positions and pixels; keeping or reordering
+        rows moves rows of the page tables only.  Without dropout on the attention probabilities:
+        the decoder has to be in eval mode."""
         fp, ct, dev = self.fp, self.ct, encoder_out.device
         d = self.d
-        if maxlen > 64:
+        paged = maxlen > 64 if paged is None else paged
+        if maxlen > 64 and not paged:
             raise ValueError("step-wise decode: at most 64 positions (attention kernel tile)")
+        if paged and self.dec.training and self.dec.dropout_p > 0:
+            raise ValueError("paged decode: no dropout on the attention probabilities, call eval() first")
+        if paged and maxlen > self.dec.pos_encoding.pe.numel() // d:
+            raise ValueError(f"paged decode: {maxlen} positions, but the positional encoding has "
+                             f"{self.dec.pos_encoding.pe.numel() // d}")
         B = encoder_out.size(0)
         enc = encoder_out.reshape(B, -1, self.E).to(ct).contiguous()
         P = enc.size(1)
@@ -253,13 +295,37 @@ class TransformerEngine:
             wq = fp.w(self._lw(i, "multihead_attn.in_proj_weight"))
             bq = fp.f32(self._lw(i, "multihead_attn.in_proj_bias"))
             kv_mem.append(K.gemm(mem, wq[d:], trans_b=True, bias=bq[d:]).view(B, P, 2 * d))
-            cache.append(torch.empty(B, maxlen, 3 * d, device=dev, dtype=ct))
+            if not paged:
+                cache.append(torch.empty(B, maxlen, 3 * d, device=dev, dtype=ct))
         seed = self.seed + 7919 * self.step_id
         self.step_id += 1
-        return dict(B=B, P=P, t=0, maxlen=maxlen, kv_mem=kv_mem, cache=cache, seed=seed)
+        st = dict(B=B, P=P, t=0, maxlen=maxlen, kv_mem=kv_mem, cache=cache, seed=seed, paged=paged)
+        if paged:
+            i32 = dict(device=dev, dtype=torch.int32)
+            pool = B * maxlen
+            st.update(pages=torch.empty(self.layers, 2, pool, 1, self.H, 64, device=dev, dtype=ct),
+                      table=torch.full((B, maxlen), -1, **i32), lens=torch.zeros(B, **i32), ones=torch.ones(B, **i32),
+                      free=torch.arange(pool - 1, -1, -1, **i32), count=torch.full((1,), pool, **i32), taken=0, plan=None,
+                      mem_table=torch.arange(B * P, **i32).view(B, P), mem_lens=torch.full((B,), P, **i32))
+        return st
 
     def decode_select(self, st, idx):
         """Keep / reorder decoding rows with their caches (beam search: caption.py:229-248)."""
+        if st["paged"]:  # rows that stem from one row share its pages
+            for name in ("table", "lens", "mem_table"):
+                st[name] = st[name].index_select(0, idx)
+            B, P, dev = idx.numel(), st["P"], st["table"].device
+            st["B"], st["plan"] = B, None
+            st["ones"] = torch.ones(B, device=dev, dtype=torch.int32)
+            st["mem_lens"] = torch.full((B,), P, device=dev, dtype=torch.int32)
+            need = st["taken"] + B * (st["maxlen"] - st["t"])
+            if need > st["free"].numel():  # more rows than at first: pages are taken in order, so the pool only grows
+                pages = st["pages"]
+                st["pages"] = torch.empty(*pages.shape[:2], need, *pages.shape[3:], device=dev, dtype=pages.dtype)
+                st["pages"][:, :, :st["taken"]] = pages[:, :, :st["taken"]]
+                st["free"] = torch.arange(need - 1, -1, -1, device=dev, dtype=torch.int32)
+                st["count"] = torch.full((1,), need - st["taken"], device=dev, dtype=torch.int32)
+            return
         st["kv_mem"] = [m.index_select(0, idx).contiguous() for m in st["kv_mem"]]
         st["cache"] = [c.index_select(0, idx).contiguous() for c in st["cache"]]
         st["B"] = idx.numel()
@@ -281,28 +347,47 @@ class TransformerEngine:
         lse = torch.empty(B, self.H, 1, device=dev, dtype=torch.float32)
         # the new position's input: embedding(last token) + pe[t]                  :129-130
         K.embedding_fwd(ids, fp.f32("embedding.weight"), x, pe=pe, L=1, drop_p=p, seed=seed, drop_stream=_S_EMB)
+        paged = st["paged"]
+        if paged:
+            if p > 0 or self.cross_probs is not None:
+                raise ValueError("paged decode: neither dropout nor recorded attention probabilities")
+            o3 = o.view(B, self.H, 64)
+            st["plan"] = K.paged_plan(st["lens"], st["ones"], st["table"], st["free"], st["count"], 1, B, out=st["plan"])
+            st["lens"], slots = st["plan"][0], st["plan"][2]
+            st["taken"] += B
         for i in range(self.layers):
             lw = lambda n: self._lw(i, n)  # noqa: E731
-            c = st["cache"][i]
-            K.gemm(x, fp.w(lw("self_attn.in_proj_weight")), trans_b=True, bias=fp.f32(lw("self_attn.in_proj_bias")),
-                   out=c[:, t])                                                 # q, k, v of position t
-            # Lq = 1: the query "row stride" ldq is the cache's batch stride
-            self._mha(B=B, Lq=1, Lk=t + 1, q=c[:, t], ldq=maxlen * 3 * d, k=c[:, :, d:], ldk=3 * d, v=c[:, :, 2 * d:],
-                      ldv=3 * d, o=o, ldo=d, lse=lse, causal=False, key_ids=None, pad_id=0, p=p, seed=seed,
-                      sid=_s(i, 0), kv_rows=maxlen)
+            if paged:
+                kc, vc = st["pages"][i]
+                q, k, v = K.gemm(x, fp.w(lw("self_attn.in_proj_weight")), trans_b=True,
+                                 bias=fp.f32(lw("self_attn.in_proj_bias"))).view(B, 3, self.H, 64).unbind(1)
+                K.paged_write(k, v, kc, vc, slots)
+                K.paged_attention(q, kc, vc, st["table"], st["lens"], max_len=t + 1, out=o3)
+            else:
+                c = st["cache"][i]
+                K.gemm(x, fp.w(lw("self_attn.in_proj_weight")), trans_b=True,
+                       bias=fp.f32(lw("self_attn.in_proj_bias")), out=c[:, t])   # q, k, v of position t
+                # Lq = 1: the query "row stride" ldq is the cache's batch stride
+                self._mha(B=B, Lq=1, Lk=t + 1, q=c[:, t], ldq=maxlen * 3 * d, k=c[:, :, d:], ldk=3 * d,
+                          v=c[:, :, 2 * d:], ldv=3 * d, o=o, ldo=d, lse=lse, causal=False, key_ids=None, pad_id=0,
+                          p=p, seed=seed, sid=_s(i, 0), kv_rows=maxlen)
             y = K.gemm(o, fp.w(lw("self_attn.out_proj.weight")), trans_b=True, bias=fp.f32(lw("self_attn.out_proj.bias")))
             x1, _, _ = K.add_layernorm(x, y, fp.f32(lw("norm1.weight")), fp.f32(lw("norm1.bias")), 1e-5,
                                        drop_p=p, seed=seed, drop_stream=_s(i, 1))
             wq = fp.w(lw("multihead_attn.in_proj_weight"))
             bq = fp.f32(lw("multihead_attn.in_proj_bias"))
             q2 = K.gemm(x1, wq[:d], trans_b=True, bias=bq[:d])
-            kv2 = st["kv_mem"][i].view(B * P, 2 * d)
-            pr = None
-            if self.cross_probs is not None:
-                pr = torch.empty(B, self.H, 1, P, device=dev, dtype=torch.float32)
-                self.cross_probs.append(pr)
-            self._mha(B=B, Lq=1, Lk=P, q=q2, ldq=d, k=kv2, ldk=2 * d, v=kv2[:, d:], ldv=2 * d, o=o, ldo=d,
-                      lse=lse, causal=False, key_ids=None, pad_id=0, p=p, seed=seed, sid=_s(i, 2), probs=pr)
+            if paged:  # every pixel a page, an image's rows sharing them
+                km, vm = st["kv_mem"][i].view(-1, 1, 2, self.H, 64).unbind(2)
+                K.paged_attention(q2.view(B, self.H, 64), km, vm, st["mem_table"], st["mem_lens"], max_len=P, out=o3)
+            else:
+                kv2 = st["kv_mem"][i].view(B * P, 2 * d)
+                pr = None
+                if self.cross_probs is not None:
+                    pr = torch.empty(B, self.H, 1, P, device=dev, dtype=torch.float32)
+                    self.cross_probs.append(pr)
+                self._mha(B=B, Lq=1, Lk=P, q=q2, ldq=d, k=kv2, ldk=2 * d, v=kv2[:, d:], ldv=2 * d, o=o, ldo=d,
+                          lse=lse, causal=False, key_ids=None, pad_id=0, p=p, seed=seed, sid=_s(i, 2), probs=pr)
             y2 = K.gemm(o, fp.w(lw("multihead_attn.out_proj.weight")), trans_b=True,
                         bias=fp.f32(lw("multihead_attn.out_proj.bias")))
             x2, _, _ = K.add_layernorm(x1, y2, fp.f32(lw("norm2.weight")), fp.f32(lw("norm2.bias")), 1e-5,
