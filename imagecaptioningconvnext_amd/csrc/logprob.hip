@@ -36,11 +36,12 @@ constexpr float LOG2E = 1.44269504088896341f, LN2 = 0.69314718055994531f;
 // of the row is in it.
 template <typename T> struct Row {
   static constexpr int VEC = 16 / sizeof(T);
-  const uint4* base;
+  const char* base;
   int skew, nvec, V;
+  DEV uint4 at(int q) const { return *(const uint4*)(base + (uint32_t)q * 16u); }  // rows end below 2^32 bytes
   DEV Row(const T* x, int V_) : V(V_) {
     skew = (int)(((uintptr_t)x & 15) / sizeof(T));
-    base = (const uint4*)((const char*)x - skew * sizeof(T));
+    base = (const char*)x - skew * sizeof(T);
     nvec = (V + skew + VEC - 1) / VEC;
   }
   // -inf in the places of vector q outside the row (the first and the last vector can have such);
@@ -74,27 +75,22 @@ template <typename T> DEV void unpack(const uint4& u, float (&v)[16 / sizeof(T)]
   }
 }
 
-// wave-wide maximum / sum on lane-permuting moves (row_shr 1, 2, 4, 8 within 16 lanes, then
-// row_bcast 15 and 31): the result of lane 63, the same for all
-template <typename F> DEV float wave_fold(float v, float none, F f) {
-#define LP_STEP(ctrl, rows)                                                                                            \
-  v = f(v, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none),                        \
-                                                                 __builtin_bit_cast(int, v), ctrl, rows, 0xf, false)))
-  LP_STEP(0x111, 0xf);
-  LP_STEP(0x112, 0xf);
-  LP_STEP(0x114, 0xf);
-  LP_STEP(0x118, 0xf);
-  LP_STEP(0x142, 0xa);
-  LP_STEP(0x143, 0xc);
-#undef LP_STEP
-  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
-}
-DEV float wave_all_max(float v) {
-  return wave_fold(v, -INFINITY, [](float a, float b) { return fmaxf(a, b); });
-}
-DEV float wave_all_sum(float v) {
-  return wave_fold(v, 0.f, [](float a, float b) { return a + b; });
-}
+// Wave-wide maximum / sum, one instruction a step: row_shr 1, 2, 4, 8 within 16 lanes, then row_bcast
+// 15 and 31; a lane without a source keeps its value, lane 63 has the result, and all get it.  (Waits:
+// two states between writing a register and a permuted read of it.)
+#define LP_FOLD(op)                                                   \
+  asm("s_nop 1\n\t" op " %0, %0, %0 row_shr:1\n\t"                    \
+      "s_nop 1\n\t" op " %0, %0, %0 row_shr:2\n\t"                    \
+      "s_nop 1\n\t" op " %0, %0, %0 row_shr:4\n\t"                    \
+      "s_nop 1\n\t" op " %0, %0, %0 row_shr:8\n\t"                    \
+      "s_nop 1\n\t" op " %0, %0, %0 row_bcast:15 row_mask:0xa\n\t"    \
+      "s_nop 1\n\t" op " %0, %0, %0 row_bcast:31 row_mask:0xc\n\t"    \
+      "s_nop 1"                                                       \
+      : "+v"(v));                                                     \
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63))
+DEV float wave_all_max(float v) { LP_FOLD("v_max_f32_dpp"); }
+DEV float wave_all_sum(float v) { LP_FOLD("v_add_f32_dpp"); }
+#undef LP_FOLD
 // the lanes' parts (reference c, -inf: nothing yet; sum s, weighted sum t) as one, in every lane; a
 // difference that passes the float range weighs nothing
 DEV void lp_join_lanes(float& c, float& s, float& t) {
@@ -120,7 +116,7 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
                                                              float* __restrict__ entropy, float* __restrict__ stats,
                                                              float* __restrict__ top_logp, int64_t* __restrict__ top_ids) {
   constexpr int VEC = 16 / sizeof(T), NW = TPB / 64, NV = 8, SEG = TPB * NV;
-  __shared__ float part[NW][4];
+  __shared__ float part[NW][3];
   __shared__ float lane_max[NW][64];
   __shared__ uint64_t cand[LP_CAND];
   __shared__ int ncand, nbusy;
@@ -137,7 +133,7 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
   uint4 u[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j)  // all in flight before the first is used: under no branch, the end again where past it
-    u[j] = r.base[min(j * TPB + tid, r.nvec - 1)];
+    u[j] = r.at(min(j * TPB + tid, r.nvec - 1));
   if (tid == 0) r.trim(u[0], 0);
   for (int q0 = 0; q0 < (LONG ? r.nvec : 1); q0 += SEG) {
     const int last = r.nvec - 1 - q0;
@@ -166,36 +162,41 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
           t = fmaf(p, fmaxf(z, -200.f), t);  // p is 0 long before -200: a finite factor beside it
         }
       }
-      if (LONG) u[j] = r.base[min(q0 + SEG + j * TPB + tid, r.nvec - 1)];  // its place in the next segment
+      if (LONG) u[j] = r.at(min(q0 + SEG + j * TPB + tid, r.nvec - 1));  // its place in the next segment
       __builtin_amdgcn_sched_barrier(0);  // one vector's floats at a time: more of them at once only spill
     }
   }
-  const float xt = hit ? to_f(x[k]) : 0.f;
+  const float xt = hit && w == 0 ? to_f(x[k]) : 0.f;
   lane_max[w][lane] = m;
-  const float wm = wave_all_max(m);
   lp_join_lanes(c, s, t);
   if (lane == 0) {
-    part[w][0] = wm;
-    part[w][1] = c;
-    part[w][2] = s;
-    part[w][3] = t;
+    part[w][0] = c;
+    part[w][1] = s;
+    part[w][2] = t;
   }
   __syncthreads();
-  float C = lane < NW ? part[lane][1] : -INFINITY, S = lane < NW ? part[lane][2] : 0.f, Z = lane < NW ? part[lane][3] : 0.f;
-  const float M = wave_all_max(lane < NW ? part[lane][0] : -INFINITY);
-  lp_join_lanes(C, S, Z);
-  const bool none = S == 0.f;  // every logit -inf
-  const float ls2 = log2f(S), l2 = none ? 0.f : fmaf(C - M, LOG2E, ls2), ls = l2 * LN2;
-  if (tid == 0) {
-    stats[2 * row] = M;
-    stats[2 * row + 1] = l2;
-    entropy[row] = none ? 0.f : (ls2 - Z / S) * LN2;
-    if (tgt) logp[row] = !hit ? 0.f : none ? -INFINITY : (xt - M) - ls;
+  float lm = lane_max[0][lane];
+#pragma unroll
+  for (int i = 1; i < NW; ++i) lm = fmaxf(lm, lane_max[i][lane]);
+  // the first wave joins the parts and puts out what is one to a row
+  float M = 0.f, ls = 0.f;
+  bool none = false;
+  if (w == 0) {
+    float C = lane < NW ? part[lane][0] : -INFINITY, S = lane < NW ? part[lane][1] : 0.f, Z = lane < NW ? part[lane][2] : 0.f;
+    M = wave_all_max(lm);
+    lp_join_lanes(C, S, Z);
+    none = S == 0.f;  // every logit -inf
+    const float ls2 = log2f(S), l2 = none ? 0.f : fmaf(C - M, LOG2E, ls2);
+    ls = l2 * LN2;
+    if (lane == 0) {
+      stats[2 * row] = M;
+      stats[2 * row + 1] = l2;
+      entropy[row] = none ? 0.f : (ls2 - Z / S) * LN2;
+      if (tgt) logp[row] = !hit ? 0.f : none ? -INFINITY : (xt - M) - ls;
+    }
   }
   if (top == 0) return;
   // the largest 16-bit key that at least `top` of the 64 partial maxima reach
-  float lm = lane_max[0][lane];
-  for (int i = 1; i < NW; ++i) lm = fmaxf(lm, lane_max[i][lane]);
   const uint32_t key = order_key(lm) >> 16;
   uint32_t bar = 0;
 #pragma unroll
@@ -212,7 +213,7 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
     const int q = busy[i0 / per] + i0 % per * TPB;
     if (q < r.nvec) {
       float v[VEC], mx = -INFINITY;
-      unpack<T>(r.base[q], v);
+      unpack<T>(r.at(q), v);
 #pragma unroll
       for (int e = 0; e < VEC; ++e) mx = fmaxf(mx, v[e]);
       if (mx < least) continue;
@@ -230,7 +231,8 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
   __syncthreads();
   const int nc = ncand;
   if (nc >= top && nc <= LP_CAND) {
-    for (int i = tid; i < nc; i += TPB) {
+    if (w > 0) return;
+    for (int i = lane; i < nc; i += 64) {
       const uint64_t mine = cand[i];
       int rank = 0;
       for (int o = 0; o < nc; ++o) rank += cand[o] > mine;
@@ -293,7 +295,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(int V, int bloc
   uint4 u[STEPS];
 #pragma unroll
   for (int j = 0; j < STEPS; ++j)
-    if (q0 + 256 * j < r.nvec) u[j] = r.base[q0 + 256 * j];
+    if (q0 + 256 * j < r.nvec) u[j] = r.at(q0 + 256 * j);
 #pragma unroll
   for (int j = 0; j < STEPS; ++j) {
     const int q = q0 + 256 * j, c0 = q * VEC - r.skew;
@@ -337,7 +339,7 @@ static int lp_check(const imgcap_logprob_desc* d, const char* name) {
   const std::string at = std::string(name) + ": ";
   IMGCAP_REQUIRE(d != nullptr, at + "desc NULL");
   IMGCAP_REQUIRE(d->dtype == IMGCAP_F32 || d->dtype == IMGCAP_BF16, at + "dtype must be fp32 or bf16");
-  IMGCAP_REQUIRE(d->n >= 0 && d->V > 0 && (d->n <= 1 || d->ld >= d->V), at + "bad n / V / ld");
+  IMGCAP_REQUIRE(d->n >= 0 && d->V > 0 && d->V <= (1 << 28) && (d->n <= 1 || d->ld >= d->V), at + "bad n / V / ld");
   return 0;
 }
 

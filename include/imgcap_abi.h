@@ -588,7 +588,7 @@ int imgcap_paged_attention_ws(const imgcap_paged_attn_desc* d, int64_t* bytes);
 int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream);
 
 /* Log-probability of given tokens, entropy and the `top` (0 .. min(64, V)) best alternatives of
- * logit rows [n, V] (pitch ld): logp[n] (0 where the target is outside [0, V); targets may be NULL),
+ * logit rows [n, V] (pitch ld, V up to 2^28): logp[n] (0 where the target is outside [0, V); targets may be NULL),
  * entropy[n] in nats, stats[n, 2] = (maximum, log2 of the sum of e^(x - maximum)) for the backward,
  * top_logp / top_ids [n, top] in falling order, ties to the lower index, NaN last.  Logits of -inf
  * have no weight; a row of them alone gives logp -inf and entropy 0.
