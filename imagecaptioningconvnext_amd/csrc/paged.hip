@@ -687,6 +687,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc 
   if (n <= chunk) return;
   const int ns = (n + chunk - 1) / chunk, w = threadIdx.x >> 6;
   const float* ml = ws_ml + (long)row * nsplit * 2;
+  const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
+  const float* oo = ws_o + (long)row * nsplit * DH + c0 + 4 * c4;
+  constexpr int AHEAD = 8;  // outputs on their way while the factors are worked out
+  f32x4 early[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i) early[i] = *(const f32x4*)(oo + (long)min(pt + i * PARTS, ns - 1) * DH);
   float M = -INFINITY, L = 0.f;
   for (int s = threadIdx.x; s < ns; s += 256) M = fmaxf(M, ml[2 * s]);
   M = wave_max(M);
@@ -703,11 +709,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc 
   if ((threadIdx.x & 63) == 0) red[4 + w] = L;
   __syncthreads();
   L = (red[4] + red[5]) + (red[6] + red[7]);
-  const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
-  const float* oo = ws_o + (long)row * nsplit * DH + c0 + 4 * c4;
   f32x4 o = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (pt + i * PARTS < ns) o += factor[pt + i * PARTS] * early[i];
 #pragma unroll 4
-  for (int s = pt; s < ns; s += PARTS) o += factor[s] * *(const f32x4*)(oo + (long)s * DH);
+  for (int s = pt + AHEAD * PARTS; s < ns; s += PARTS) o += factor[s] * *(const f32x4*)(oo + (long)s * DH);
   part[pt][c4] = o;
   __syncthreads();
   if (threadIdx.x < COLS) {
