@@ -743,10 +743,12 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
                  "paged attention: max_len must be within the table's width, and that at most 2^31 - 65536 tokens");
   IMGCAP_REQUIRE(d->q && d->k && d->v && d->o && d->table && d->lens, "paged attention: NULL operand");
   const int64_t vec = d->dtype == IMGCAP_F32 ? 4 : 8;
-  IMGCAP_REQUIRE(aligned16(d->q) && aligned16(d->k) && aligned16(d->v) && d->q_row % vec == 0 && d->q_head % vec == 0 &&
-                     d->k_page % vec == 0 && d->k_tok % vec == 0 && d->k_head % vec == 0 && d->v_page % vec == 0 &&
-                     d->v_tok % vec == 0 && d->v_head % vec == 0,
-                 "paged attention: q, k and v must be 16-byte aligned with strides of whole 16 bytes");
+  const struct { int size; int64_t stride; } dims[] = {{d->B, d->q_row},      {d->H, d->q_head},  {d->pages, d->k_page},
+                                                       {d->page, d->k_tok},   {d->Hkv, d->k_head}, {d->pages, d->v_page},
+                                                       {d->page, d->v_tok},   {d->Hkv, d->v_head}};
+  bool whole = aligned16(d->q) && aligned16(d->k) && aligned16(d->v);
+  for (const auto& m : dims) whole = whole && (m.size <= 1 || m.stride % vec == 0);  // no stride where there is one of it
+  IMGCAP_REQUIRE(whole, "paged attention: q, k and v must be 16-byte aligned with strides of whole 16 bytes");
   return 0;
 }
 
@@ -854,9 +856,11 @@ extern "C" int imgcap_paged_write(const imgcap_paged_write_desc* d, void* stream
                  "imgcap_paged_write: page must be a power of two, at most 1024");
   if (d->n == 0) return 0;
   IMGCAP_REQUIRE(d->k && d->v && d->kc && d->vc && d->slots, "imgcap_paged_write: NULL operand");
-  const int64_t st[] = {d->k_row, d->k_head, d->v_row, d->v_head, d->kc_page, d->kc_tok, d->kc_head, d->vc_page,
-                        d->vc_tok, d->vc_head};
-  for (int64_t s : st) IMGCAP_REQUIRE(s % vec == 0, "imgcap_paged_write: strides must be whole 16-byte pieces");
+  const struct { int size; int64_t stride; } dims[] = {
+      {d->n, d->k_row},      {d->heads, d->k_head},  {d->n, d->v_row},      {d->heads, d->v_head},  {d->pages, d->kc_page},
+      {d->page, d->kc_tok},  {d->heads, d->kc_head}, {d->pages, d->vc_page}, {d->page, d->vc_tok},  {d->heads, d->vc_head}};
+  for (const auto& m : dims)
+    IMGCAP_REQUIRE(m.size <= 1 || m.stride % vec == 0, "imgcap_paged_write: strides must be whole 16-byte pieces");
   IMGCAP_REQUIRE(aligned16(d->k) && aligned16(d->v) && aligned16(d->kc) && aligned16(d->vc),
                  "imgcap_paged_write: operands must be 16-byte aligned");
   const int vecs = d->dh / vec;

@@ -666,7 +666,8 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     (imgcap_paged_plan): request b, with past[b] tokens in the cache, gets new[b] more, or has ended
     (new[b] < 0: its pages go back).  ``table`` [B, width] int32 gets the new pages' ids, which come
     from the end of the stack ``free`` [pool] int32 holding ``count`` [1] int32 of them; the number
-    left goes to ``count_out`` (default: count itself).  ``tokens`` is the step's capacity, at least
+    left goes to ``count_out`` (default: count itself).  ``page``, tokens a page, is a power of two up to
+    1024 (1: slots are pages, and rows that stem from one row may share them).  ``tokens`` is the step's capacity, at least
     the sum of new.  Returns (lens [B] int32, starts [B + 1] int32, slots [tokens] int64, rows
     [tokens] int32, positions [tokens] int64, waits [B] int32); pass it back as ``out`` to have it
     filled again (a captured graph's outputs); ``past`` may be its lens, so that a loop's lengths go on
@@ -680,12 +681,13 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     i32, i64 = torch.int32, torch.int64
     _want(name, "past", past, i32, (B,))
     _want(name, "new", new, i32, (B,))
-    _want(name, "free", free, i32, (free.numel(),))
+    pool = free.numel()
+    if not (0 < page <= 1024 and 0 <= tokens < 1 << 31 and pool < 1 << 31):  # the C side's integers have 32 bits
+        raise ValueError(f"paged_plan: page {page}, tokens {tokens} or pool {pool} out of range")
+    _want(name, "free", free, i32, (pool,))
     _want(name, "count", count, i32, (1,))
     _want(name, "count_out", count_out, i32, (1,))
     if out is None:
-        if tokens < 0:
-            raise ValueError(f"paged_plan: tokens must not be negative, got {tokens}")
         out = (past.new_empty(B), past.new_empty(B + 1), past.new_empty(tokens, dtype=i64), past.new_empty(tokens),
                past.new_empty(tokens, dtype=i64), past.new_empty(B))
         lens, starts, slots, rows, positions, waits = out
@@ -699,7 +701,7 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
         _want(name, "positions", positions, i64, (tokens,))
         _want(name, "waits", waits, i32, (B,))
     ws = None if B <= _PLAN_ROWS and tokens <= _PLAN_TOKENS and width <= _PLAN_CAP else past.new_empty(B + 1)
-    d = _abi.PagedPlanDesc(B, width, page, free.numel(), tokens, table_row, past.data_ptr(), new.data_ptr(),
+    d = _abi.PagedPlanDesc(B, width, page, pool, tokens, table_row, past.data_ptr(), new.data_ptr(),
                            table.data_ptr(), free.data_ptr(), count.data_ptr(), count_out.data_ptr(), lens.data_ptr(),
                            starts.data_ptr(), slots.data_ptr(), rows.data_ptr(), positions.data_ptr(),
                            waits.data_ptr(), ptr(ws))
@@ -747,7 +749,8 @@ def paged_write(k, v, k_cache, v_cache, slots):
 def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=None, out=None, lse=None):
     """Attention of one new token per request over its pages (imgcap_paged_attention): q [B, H, head
     dim], caches [pages, page, kv heads, head dim] of any strides, table [B, width] int32, lens [B]
-    int32 -> out [B, H, head dim].  H is a multiple of the kv heads, head dim 64 or 128, fp32 or bf16.
+    int32 -> out [B, H, head dim] (q itself may be given).  H is a multiple of the kv heads, head dim 64
+    or 128, pages a power of two up to 1024 tokens, fp32 or bf16.
     ``max_len`` (default: the table's width) bounds the lengths from the host; the work is cut for it.
     A request of length 0 gets zeros; positions on a page outside the cache are not there.
     ``lse`` [B, H] fp32 gets the natural log-sum-exp of the scores (default scale: head dim ** -0.5)."""
@@ -773,7 +776,11 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
         _want(name, "lse", lse, torch.float32, (B, H))
     if B == 0:
         return out
-    d = _abi.PagedAttnDesc(dt(q), B, H, hkv, dh, page, pages, width, width * page if max_len is None else max_len,
+    if max_len is None:
+        max_len = width * page
+    elif not 0 < max_len <= width * page:
+        raise ValueError(f"paged_attention: max_len {max_len} must be in 1 .. {width * page}, the table's width")
+    d = _abi.PagedAttnDesc(dt(q), B, H, hkv, dh, page, pages, width, max_len,
                            dh ** -0.5 if scale is None else scale, qs[0], qs[1], os_[0], os_[1], ks[0], ks[1], ks[2],
                            vs[0], vs[1], vs[2], table_row, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                            out.data_ptr(), ptr(lse), table.data_ptr(), lens.data_ptr(), None, 0)

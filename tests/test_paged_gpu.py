@@ -197,14 +197,17 @@ def test_attention_scale(hip_device, scale):
     _check(torch.randn(2, 2, 128, device=hip_device), kc, vc, table, [50, 3], scale=scale)
 
 
-def test_attention_far_offsets(hip_device):
+@pytest.mark.parametrize("page", [64, 1])
+def test_attention_far_offsets(hip_device, page):
     """A cache of more than 2^31 elements: pages at its end are where they should be."""
     dev = hip_device
-    page, hkv, dh = 64, 8, 128
-    pages = (1 << 31) // (page * hkv * dh) + 40
+    hkv, dh = 8, 128
+    pages = (1 << 31) // (page * hkv * dh) + 400
     kc, vc = (torch.zeros(pages, page, hkv, dh, dtype=BF, device=dev) for _ in range(2))
     lens, g = [100, 190], torch.Generator().manual_seed(10)
-    table = torch.tensor([[pages - 1, pages - 37, -1], [pages - 2, 3, pages - 20]], dtype=torch.int32, device=dev)
+    width = (190 + page - 1) // page
+    table = pages - 1 - torch.randperm(2 * width, generator=g).view(2, width).to(torch.int32).to(dev)
+    table[1, 1] = 3
     K = _k()
     rows = sum(lens)
     k, v = (torch.randn(rows, hkv, dh, generator=g).to(BF).to(dev) for _ in range(2))
@@ -261,11 +264,32 @@ def test_attention_refuses(hip_device):
     for bad in (dict(q=q.float()), dict(q=q[:, :3]), dict(q=q[:1]), dict(q=q[..., :32]), dict(q=q.transpose(0, 1)[:, :, ::2]),
                 dict(table=table.long()), dict(table=table[:1]), dict(table=table.t()), dict(lens=n.long()), dict(lens=n[:1]),
                 dict(v_cache=vc[:1]), dict(v_cache=vc.float()), dict(k_cache=kc[:, :12]), dict(out=q.float()),
-                dict(out=q[:1]), dict(lse=torch.zeros(2, 4, device=dev, dtype=BF)), dict(max_len=0), dict(max_len=1 << 20),
+                dict(out=q[:1]), dict(max_len=(1 << 32) + 32), dict(lse=torch.zeros(2, 4, device=dev, dtype=BF)), dict(max_len=0), dict(max_len=1 << 20),
                 dict(lens=n.cpu()), dict(q=q.half()), dict(k_cache=kc.flatten()[4:-4092].view(-1, 16, 2, 64)[:4])):
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             K.paged_attention(**{**ok, **bad})
     assert K.paged_attention(q[:0], kc, vc, table[:0], n[:0]).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dtype", [BF, F])
+def test_attention_in_place_and_single_dims(hip_device, dtype):
+    """The output may be the queries' own buffer; dimensions of one have no stride that counts."""
+    K, dev = _k(), hip_device
+    for lens, page in (([40, 2, 0], 8), ([700, 90, 3], 16), ([2600, 5, 64], 16)):
+        kc, vc, table = _cache(lens, page, 2, 64, dtype, 24, dev)
+        n = torch.tensor(lens, dtype=torch.int32, device=dev)
+        q = torch.randn(3, 40, 64, device=dev).to(dtype)
+        want = K.paged_attention(q, kc, vc, table, n)
+        assert K.paged_attention(q, kc, vc, table, n, out=q) is q and torch.equal(q, want)
+    base = torch.randn(9, 67, device=dev).to(dtype)  # rows of 67: a stride that is no whole 16 bytes
+    one = base[:1, :64].as_strided((1, 1, 1, 64), (67, 67, 67, 1))
+    q = base[1:2].as_strided((1, 1, 64), (67, 67, 1), 0)
+    got = K.paged_attention(q, one, one, torch.zeros(1, 1, dtype=torch.int32, device=dev),
+                            torch.ones(1, dtype=torch.int32, device=dev))
+    assert torch.equal(got[0, 0], one[0, 0, 0])
+    into = torch.zeros(1, 1, 1, 64, device=dev, dtype=dtype)
+    K.paged_write(q, q, into, into.clone(), torch.zeros(1, dtype=torch.int64, device=dev))
+    assert torch.equal(into[0, 0, 0], base[0, :64])
 
 
 # ---- the writer -----------------------------------------------------------------------------
@@ -424,7 +448,7 @@ def test_plan_outputs_again_and_refusals(hip_device):
     p, t, c = torch.zeros(2, **i32), torch.zeros(2, 4, **i32), torch.ones(1, **i32)
     ok = dict(past=p, new=p, table=t, free=torch.zeros(8, **i32), count=c, page=16, tokens=4)
     for bad in (dict(past=p.long()), dict(past=p[:1]), dict(table=t.t()), dict(table=t.long()), dict(count=p), dict(page=5),
-                dict(tokens=-1), dict(free=torch.zeros(0, **i32)), dict(count=c.cpu()), dict(out=first),
+                dict(tokens=-1), dict(tokens=(1 << 32) + 4), dict(page=(1 << 32) + 16), dict(free=torch.zeros(0, **i32)), dict(count=c.cpu()), dict(out=first),
                 dict(new=torch.zeros(4, **i32)[::2])):
         with pytest.raises((TypeError, ValueError, RuntimeError)):
             K.paged_plan(**{**ok, **bad})
