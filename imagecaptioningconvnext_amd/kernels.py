@@ -617,25 +617,24 @@ def transpose(x, out=None):
 # ---- paged key/value cache and token log-probabilities ------------------------------------------
 # These are calls of a few microseconds on the GPU, one after another in a decoding loop, so the
 # host side is kept to plain integers: devices as indices, the raw stream handle (0.1 us; a Stream
-# object costs 2.6), no library workspace looked after (they take none).
+# object costs 2.6), descriptors instead of single arguments, no library workspace looked after (they
+# take none), and one expression that says whether all is well before any that says what is not.
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _one_device(name, t0, *ts):
-    """Index of the GPU that all of the tensors (None left out) live on."""
-    dev = t0.get_device()
+def _mixed(name, t0, *ts):
+    """Raise: the tensors are not on one GPU."""
     for t in ts:
-        if t is not None and t.get_device() != dev:
+        if t is not None and t.device != t0.device:
             raise ValueError(f"{name}: tensors on {t0.device} and {t.device}")
-    if dev < 0:
-        raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
-    return dev
+    raise RuntimeError("imgcap kernels need GPU tensors (no CPU fallback)")
 
 
 def _run_on(dev, name, desc):
     """Return code of ``name`` on the current stream of GPU ``dev``, whichever is the current one."""
     fn = getattr(_abi.lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         return fn(desc, _raw_stream(dev))
     with torch.cuda.device(dev):
         return fn(desc, _raw_stream(dev))
@@ -675,31 +674,39 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     no page left, no token left -- waits: waits[b] = 1, nothing else of it changes."""
     name = "paged_plan"
     count_out = count if count_out is None else count_out
-    dev = _one_device(name, past, new, table, free, count, count_out)
-    B = past.numel()
+    dev = past.get_device()
+    if not (dev >= 0 and dev == new.get_device() == table.get_device() == free.get_device() == count.get_device()
+            == count_out.get_device()):
+        _mixed(name, past, new, table, free, count, count_out)
+    B, pool = past.numel(), free.numel()
     table_row, width = _int_rows(name, "table", table, B)
-    i32, i64 = torch.int32, torch.int64
-    _want(name, "past", past, i32, (B,))
-    _want(name, "new", new, i32, (B,))
-    pool = free.numel()
     if not (0 < page <= 1024 and 0 <= tokens < 1 << 31 and pool < 1 << 31):  # the C side's integers have 32 bits
         raise ValueError(f"paged_plan: page {page}, tokens {tokens} or pool {pool} out of range")
-    _want(name, "free", free, i32, (pool,))
-    _want(name, "count", count, i32, (1,))
-    _want(name, "count_out", count_out, i32, (1,))
+    i32, i64, rows_shape = torch.int32, torch.int64, (B,)
+    if not (past.dtype is new.dtype is free.dtype is count.dtype is count_out.dtype is i32 and past.shape == rows_shape
+            and new.shape == rows_shape and count.numel() == 1 and count_out.numel() == 1 and free.dim() == 1
+            and past.is_contiguous() and new.is_contiguous() and free.is_contiguous()):
+        for what, t, shape in (("past", past, rows_shape), ("new", new, rows_shape), ("free", free, (pool,)),
+                               ("count", count, (1,)), ("count_out", count_out, (1,))):
+            _want(name, what, t, i32, shape)
     if out is None:
         out = (past.new_empty(B), past.new_empty(B + 1), past.new_empty(tokens, dtype=i64), past.new_empty(tokens),
                past.new_empty(tokens, dtype=i64), past.new_empty(B))
         lens, starts, slots, rows, positions, waits = out
     else:
         lens, starts, slots, rows, positions, waits = out
-        _one_device(name, past, *out)
-        _want(name, "lens", lens, i32, (B,))
-        _want(name, "starts", starts, i32, (B + 1,))
-        _want(name, "slots", slots, i64, (tokens,))
-        _want(name, "rows", rows, i32, (tokens,))
-        _want(name, "positions", positions, i64, (tokens,))
-        _want(name, "waits", waits, i32, (B,))
+        if not (dev == lens.get_device() == starts.get_device() == slots.get_device() == rows.get_device()
+                == positions.get_device() == waits.get_device()):
+            _mixed(name, past, *out)
+        if not (lens.dtype is starts.dtype is rows.dtype is waits.dtype is i32 and slots.dtype is positions.dtype is i64
+                and lens.shape == rows_shape == waits.shape and starts.shape == (B + 1,)
+                and slots.shape == rows.shape == positions.shape == (tokens,) and lens.is_contiguous()
+                and starts.is_contiguous() and slots.is_contiguous() and rows.is_contiguous()
+                and positions.is_contiguous() and waits.is_contiguous()):
+            for what, t, dtype, n in (("lens", lens, i32, B), ("starts", starts, i32, B + 1), ("slots", slots, i64, tokens),
+                                      ("rows", rows, i32, tokens), ("positions", positions, i64, tokens),
+                                      ("waits", waits, i32, B)):
+                _want(name, what, t, dtype, (n,))
     ws = None if B <= _PLAN_ROWS and tokens <= _PLAN_TOKENS and width <= _PLAN_CAP else past.new_empty(B + 1)
     d = _abi.PagedPlanDesc(B, width, page, pool, tokens, table_row, past.data_ptr(), new.data_ptr(),
                            table.data_ptr(), free.data_ptr(), count.data_ptr(), count_out.data_ptr(), lens.data_ptr(),
@@ -711,33 +718,28 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     return out
 
 
-def _cache_pair(name, k, v):
-    if k.dim() != 4 or k.shape != v.shape:
-        raise ValueError(f"{name}: caches must be [pages, page, kv heads, head dim], both alike")
-    ks, vs = k.stride(), v.stride()
-    if ks[3] != 1 or vs[3] != 1:
-        raise ValueError(f"{name}: caches must have unit inner stride")
-    return k.shape, ks, vs
-
-
 def paged_write(k, v, k_cache, v_cache, slots):
     """k_cache[slot // page, slot % page] = k[i] for slot = slots[i] (int64, imgcap_paged_write), and
     the values alike: k / v [n, kv heads, head dim] views, caches [pages, page, kv heads, head dim] of
     any strides.  A slot outside the cache (-1: padding) is skipped.  Slots of one call are distinct."""
     name = "paged_write"
-    dev = _one_device(name, k, v, k_cache, v_cache, slots)
-    (pages, page, heads, dh), kc, vc = _cache_pair(name, k_cache, v_cache)
-    if not (k.dtype == v.dtype == k_cache.dtype == v_cache.dtype):
-        raise TypeError("paged_write: k, v and the caches must share a dtype")
+    dev = k.get_device()
+    if not (dev >= 0 and dev == v.get_device() == k_cache.get_device() == v_cache.get_device() == slots.get_device()):
+        _mixed(name, k, v, k_cache, v_cache, slots)
+    ks, vs, kc, vc = k.stride(), v.stride(), k_cache.stride(), v_cache.stride()
+    shape = k_cache.shape
+    if len(kc) != 4 or v_cache.shape != shape or kc[3] != 1 or vc[3] != 1:
+        raise ValueError("paged_write: caches must be [pages, page, kv heads, head dim], both alike, with unit inner stride")
+    pages, page, heads, dh = shape
     n = slots.numel()
-    _want(name, "slots", slots, torch.int64, (n,))
-    if k.shape != (n, heads, dh) or v.shape != (n, heads, dh):
-        raise ValueError(f"paged_write: k and v must be [{n}, {heads}, {dh}]")
+    if k.shape != (n, heads, dh) or v.shape != k.shape or ks[2] != 1 or vs[2] != 1:
+        raise ValueError(f"paged_write: k and v must be [{n}, {heads}, {dh}] with unit inner stride")
+    if not k.dtype is v.dtype is k_cache.dtype is v_cache.dtype:
+        raise TypeError("paged_write: k, v and the caches must share a dtype")
+    if slots.dtype is not torch.int64 or slots.dim() != 1 or not slots.is_contiguous():
+        _want(name, "slots", slots, torch.int64, (n,))
     if n == 0:
         return
-    ks, vs = k.stride(), v.stride()
-    if ks[2] != 1 or vs[2] != 1:
-        raise ValueError("paged_write: k and v must have unit inner stride")
     d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0],
                             vc[1], vc[2], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                             slots.data_ptr())
@@ -755,23 +757,29 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
     A request of length 0 gets zeros; positions on a page outside the cache are not there.
     ``lse`` [B, H] fp32 gets the natural log-sum-exp of the scores (default scale: head dim ** -0.5)."""
     name = "paged_attention"
-    dev = _one_device(name, q, k_cache, v_cache, table, lens, out, lse)
-    (pages, page, hkv, dh), ks, vs = _cache_pair(name, k_cache, v_cache)
-    if q.dim() != 3 or q.shape[2] != dh:
-        raise ValueError(f"paged_attention: q must be [B, H, {dh}]")
-    if not (q.dtype == k_cache.dtype == v_cache.dtype):
+    dev = q.get_device()
+    if not (dev >= 0 and dev == k_cache.get_device() == v_cache.get_device() == table.get_device() == lens.get_device()
+            and (out is None or dev == out.get_device()) and (lse is None or dev == lse.get_device())):
+        _mixed(name, q, k_cache, v_cache, table, lens, out, lse)
+    qs, ks, vs = q.stride(), k_cache.stride(), v_cache.stride()
+    shape = k_cache.shape
+    if len(ks) != 4 or v_cache.shape != shape or ks[3] != 1 or vs[3] != 1:
+        raise ValueError("paged_attention: caches must be [pages, page, kv heads, head dim], both alike, with unit inner stride")
+    pages, page, hkv, dh = shape
+    shape, dtype = q.shape, q.dtype
+    if len(qs) != 3 or shape[2] != dh or qs[2] != 1:
+        raise ValueError(f"paged_attention: q must be [B, H, {dh}] with unit inner stride")
+    if not dtype is k_cache.dtype is v_cache.dtype:
         raise TypeError("paged_attention: q and the caches must share a dtype")
-    B, H, _ = q.shape
+    B, H, _ = shape
     table_row, width = _int_rows(name, "table", table, B)
-    _want(name, "lens", lens, torch.int32, (B,))
+    if lens.dtype is not torch.int32 or lens.shape != (B,) or not lens.is_contiguous():
+        _want(name, "lens", lens, torch.int32, (B,))
     if out is None:
-        out = q.new_empty((B, H, dh))
-    else:
-        if out.dtype is not q.dtype or out.shape != q.shape:
-            raise ValueError(f"paged_attention: out must be {q.dtype} of shape {tuple(q.shape)}")
-    qs, os_ = q.stride(), out.stride()
-    if qs[2] != 1 or os_[2] != 1:
-        raise ValueError("paged_attention: q and out must have unit inner stride")
+        out = q.new_empty(shape)
+    os_ = out.stride()
+    if out.dtype is not dtype or out.shape != shape or os_[2] != 1:
+        raise ValueError(f"paged_attention: out must be {dtype} of shape {tuple(shape)} with unit inner stride")
     if lse is not None:
         _want(name, "lse", lse, torch.float32, (B, H))
     if B == 0:
@@ -814,17 +822,20 @@ def token_logprobs(logits, targets=None, V=None, *, top=0):
     outside [0, V) (-1: padding) gives logp 0.  Alternatives come in falling order, equal ones by
     index, NaN last.  Logits of -inf have no weight; a row of them alone gives -inf and entropy 0."""
     name = "token_logprobs"
-    dev = _one_device(name, logits, targets)
+    dev = logits.get_device()
+    if not (dev >= 0 and (targets is None or dev == targets.get_device())):
+        _mixed(name, logits, targets)
     n, V, ld = _logit_rows(name, logits, V)
-    f32 = torch.float32
     if not 0 <= top <= min(64, V):
         raise ValueError(f"token_logprobs: top must be in 0 .. {min(64, V)}")
-    logp = None
-    if targets is not None:
+    if targets is not None and (targets.dtype is not torch.int64 or targets.shape != (n,) or not targets.is_contiguous()):
         _want(name, "targets", targets, torch.int64, (n,))
-        logp = logits.new_empty(n, dtype=f32)
-    entropy, stats = logits.new_empty(n, dtype=f32), logits.new_empty((n, 2), dtype=f32)
-    top_logp, top_ids = logits.new_empty((n, top), dtype=f32), logits.new_empty((n, top), dtype=torch.int64)
+    entropy = logits.new_empty(n, dtype=torch.float32)
+    stats, top_logp = entropy.new_empty((n, 2)), entropy.new_empty((n, top))
+    if targets is None:
+        logp, top_ids = None, logits.new_empty((n, top), dtype=torch.int64)
+    else:
+        logp, top_ids = entropy.new_empty(n), targets.new_empty((n, top))
     d = _abi.LogprobDesc(dt(logits), n, V, top, ld, 0, logits.data_ptr(), ptr(targets), ptr(logp), entropy.data_ptr(),
                          stats.data_ptr(), top_logp.data_ptr(), top_ids.data_ptr())
     rc = _run_on(dev, "imgcap_token_logprobs", d)
@@ -838,7 +849,10 @@ def token_logprobs_bwd(logits, targets, stats, entropy, dlogp=None, dentropy=Non
     be None) -> dlogits [n, V] in the logits' dtype (of a given ``dlogits`` [n, >= V], which may be
     ``logits`` itself, the columns from V on stay).  The alternatives have no gradient."""
     name = "token_logprobs_bwd"
-    dev = _one_device(name, logits, targets, stats, entropy, dlogp, dentropy, dlogits)
+    dev = logits.get_device()
+    for t in (targets, stats, entropy, dlogp, dentropy, dlogits):
+        if dev < 0 or t is not None and t.get_device() != dev:
+            _mixed(name, logits, targets, stats, entropy, dlogp, dentropy, dlogits)
     n, V, ld = _logit_rows(name, logits, V)
     f32 = torch.float32
     if dlogp is not None and targets is None:
