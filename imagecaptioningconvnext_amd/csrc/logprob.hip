@@ -110,6 +110,10 @@ DEV void lp_join_lanes(float& c, float& s, float& t) {
 // that at least `top` elements reach; the few elements that reach it are gathered in LDS and ranked
 // there.  Where more than LP_CAND do (long ties), or too few (NaN), the alternatives are found one by
 // one, in passes over the row.
+// Bound by vector issue beside HBM: 8.4 instructions a logit (the exponential at a quarter of the rate)
+// and some 300 a wave.  MI355X: 3264 x 9490 bf16 with 5 alternatives 18.4 us (62 MB; 12.7 at the rate of
+// a large copy), 1000 x 131072 bf16 with 20 59.5 us (4.4 TB/s), 777 x 50257 fp32 with 10 35.8 us
+// (4.4 TB/s), 5 x 9490 fp32 6.1 us.
 template <typename T, int TPB, bool LONG>
 __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, const T* __restrict__ logits, long ld,
                                                              const int64_t* __restrict__ tgt, float* __restrict__ logp,
@@ -270,7 +274,8 @@ __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, con
 // memory-side cache; where logits and gradient together pass its 256 MB the stores are streaming, or
 // they push out what is still to be read (777 x 50257 fp32 forward and gradient 103 -> 86 us; 3264 x
 // 9490 bf16, 124 MB in all, 45.6 -> 44.7 by the order alone, and its stores stay cached for the
-// product that reads them next).
+// product that reads them next).  A row is cut into even shares of up to 1024 vectors: at 9490 words
+// two of 594, not 1024 and 163, 25.9 -> 20.5 us (6 TB/s of reads and writes, the reads cached).
 template <typename T>
 __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(int V, int blocks, const T* logits, long ld,
                                                                  const int64_t* __restrict__ tgt,
@@ -291,15 +296,16 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(int V, int bloc
   if (m == -INFINITY && l2 == 0.f) m = 0.f;  // every logit -inf: p = 0 throughout
   const float g = dlogp && k >= 0 && k < V ? dlogp[row] : 0.f, h = dentropy ? dentropy[row] : 0.f;
   const float a = -g - h * entropy[row], b = -h * LN2;
-  const int q0 = (blockIdx.x % blocks) * (256 * STEPS) + threadIdx.x;
+  const int per = (r.nvec + blocks - 1) / blocks, begin = (blockIdx.x % blocks) * per;  // even shares of the row
+  const int end = min(begin + per, r.nvec), q0 = begin + threadIdx.x;
   uint4 u[STEPS];
 #pragma unroll
   for (int j = 0; j < STEPS; ++j)
-    if (q0 + 256 * j < r.nvec) u[j] = r.at(q0 + 256 * j);
+    if (q0 + 256 * j < end) u[j] = r.at(q0 + 256 * j);
 #pragma unroll
   for (int j = 0; j < STEPS; ++j) {
     const int q = q0 + 256 * j, c0 = q * VEC - r.skew;
-    if (q >= r.nvec) break;
+    if (q >= end) break;
     float v[VEC];
     unpack<T>(u[j], v);
 #pragma unroll
@@ -352,6 +358,9 @@ extern "C" int imgcap_token_logprobs(const imgcap_logprob_desc* d, void* stream)
                      (top == 0 || (d->top_logp && d->top_ids)),
                  "imgcap_token_logprobs: NULL operand");
   hipStream_t st = (hipStream_t)stream;
+  // Few rows: 1024 threads each, for latency (5 x 9490 6.1 us).  More than 512: 256 threads for rows that
+  // these hold in registers or nearly (3264 x 9490 22 us, 30 with 512), 512 beyond (1280 x 50257 fp32
+  // 50.4 us, 53.4 with 256; 1000 x 131072 bf16 61, 64 with 256).
 #define LP_(T, TPB, LONG)                                                                                 \
   hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, LONG>), dim3(n), dim3(TPB), 0, st, V, top,            \
                      (const T*)d->logits, (long)d->ld, d->targets, d->logp, d->entropy, d->stats, d->top_logp, d->top_ids)
