@@ -400,7 +400,8 @@ extern "C" int imgcap_token_logprobs_bwd(const imgcap_logprob_desc* d, void* str
     const int vec = 16 / (int)sizeof(T), blocks = ((V + 2 * vec - 2) / vec + 1023) / 1024;                          \
     IMGCAP_REQUIRE((int64_t)n * blocks < (1ll << 31), "imgcap_token_logprobs_bwd: too many rows");                  \
     hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3((unsigned)n * blocks), dim3(256), 0, st, V, blocks,       \
-                       (const T*)d->logits, (long)d->ld, d->targets, d->stats, d->entropy, d->dlogp, d->dentropy, (T*)d->dlogits, (long)d->ldd, \
+                       (const T*)d->logits, (long)d->ld, d->targets, d->stats, d->entropy, d->dlogp,                \
+                       d->dentropy, (T*)d->dlogits, (long)d->ldd,                                                   \
                        (int64_t)n * V * (int64_t)sizeof(T) > (128ll << 20) ? 1 : 0);                                \
   } while (0)
   if (d->dtype == IMGCAP_BF16) LPB_(bf16);

@@ -15,8 +15,8 @@ namespace imgcap {
 // lengths and the stack's height; then the pages that requests have open, the top of the stack and the
 // pages of ended requests, all of which the tokens find in LDS.  Barriers wait for LDS alone, not for
 // the global stores and loads on their way (64 requests, five of them ended: 3.2 us; with a pass over
-// the requests' pages and loads one after another 8.2).  More tokens go to a second launch over the whole chip; more requests (or sums that might
-// pass 32 bits) to a pass in chunks with 64-bit sums.
+// the requests' pages and loads one after another 8.2).  More tokens go to a second launch over the
+// whole chip; more requests (or sums that might pass 32 bits) to a pass in chunks with 64-bit sums.
 constexpr int PLAN_ROWS = 1024, PLAN_TOKENS = 4096, PLAN_CAP = 1 << 20, PLAN_BACK = 2048;
 
 struct PlanArgs : imgcap_paged_plan_desc { int lp; };  // lp: log2 of the page size
@@ -253,8 +253,9 @@ __global__ __launch_bounds__(1024) void paged_plan_long_kernel(PlanArgs a) {
 
 // lays out the tokens after either planner: four consecutive ones a thread (one search for them, 16-byte
 // stores where the outputs are so aligned), the starts in LDS if they fit.  Bound by latency and the
-// 20 bytes a token that it writes (500,250 tokens of 500 requests 7.4 us; a token a thread 9.4).  A request's old length is its new one less its tokens (past itself may
-// be the array that the new ones went to).
+// 20 bytes a token that it writes (500,250 tokens of 500 requests 7.4 us; a token a thread 9.4).  A
+// request's old length is its new one less its tokens (past itself may be the array that the new ones
+// went to).
 constexpr int SLOT_TOKENS = 1024, SLOT_ROWS = 4096;
 __global__ __launch_bounds__(256) void paged_slots_kernel(PlanArgs a, int aligned) {
   __shared__ int32_t starts_s[SLOT_ROWS];
@@ -453,12 +454,13 @@ DEV uint32_t pack_bf16(float a, float b) {
 }
 
 // JOIN: the workgroup's waves share a chunk (blockIdx.x the row, blockIdx.y the chunk), 32 tokens each
-// in turn, and put their parts together in LDS.  Else each wave has a row and chunk to itself, the
-// waves of a group consecutive rows (kv heads of the same tokens, which lie side by side in memory),
-// and nothing is exchanged.  Bound by HBM where the caches are large, and more waves than two a SIMD
+// in turn, and put their parts together in LDS.  Else each wave has a short row to itself, the waves of
+// a group consecutive rows (kv heads of the same tokens, which lie side by side in memory), and
+// nothing is exchanged.  Bound by HBM where the caches are large, and more waves than two a SIMD
 // only lengthen the queues there (first scores of a wave after 16 us at 12 waves a CU): 48 requests of
 // up to 20011 tokens 393 us at two, 401 at three.
 constexpr int JOIN_WAVES = 4, MAX_SPLIT = 1024;
+static_assert(JOIN_WAVES % 2 == 0, "half of the waves hand over to the other half");
 template <typename T, int DH, bool TINY, bool JOIN>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void paged_attn_kernel(
     imgcap_paged_attn_desc d, int chunk, int nsplit, int gtiles, int lp, float* ws_o, float* ws_ml) {
@@ -595,29 +597,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     }
   }
   l = groups_fold(l, [](float x, float y) { return x + y; });
-  const bool whole = n <= chunk;
   // lane (r, g) holds head r, columns VPL * (4 g + i) + j: DH / 4 consecutive ones
-  if constexpr (!JOIN) {
+  if constexpr (!JOIN) {  // rows that are not split
     if (r >= heads) return;
-    const long bh = (long)b * d.H + h0 + r;
-    if (whole) {
-      const float f = l == 0.f ? 0.f : 1.f / l;
-      T* o = (T*)d.o + (long)b * d.o_row + (long)(h0 + r) * d.o_head + VPL * 4 * g;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+    T* o = (T*)d.o + (long)b * d.o_row + (long)(h0 + r) * d.o_head + VPL * 4 * g;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int j = 0; j < VPL; ++j) o[VPL * i + j] = from_f<T>(l == 0.f ? 0.f : acc[j][i] * f);
-      if (d.lse && g == 0) d.lse[bh] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
-    } else {
-      float* o = ws_o + (bh * nsplit + split) * DH + VPL * 4 * g;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < VPL; j += 4)
-          *(f32x4*)(o + VPL * i + j) = f32x4{acc[j][i], acc[j + 1][i], acc[j + 2][i], acc[j + 3][i]};
-      if (g == 0) *(f32x2*)(ws_ml + (bh * nsplit + split) * 2) = f32x2{m, l};
-    }
+      for (int j = 0; j < VPL; ++j) o[VPL * i + j] = from_f<T>(l == 0.f ? 0.f : acc[j][i] * f);
+    if (d.lse && g == 0) d.lse[(long)b * d.H + h0 + r] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
   } else {
+    const bool whole = n <= chunk;
     __shared__ float ml[JOIN_WAVES][2][16];
     __shared__ float sm[JOIN_WAVES / 2 * 16 * LDO];  // parts, to the common maximum
     if (g == 0) {
@@ -632,7 +623,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
     for (int i = 0; i < JOIN_WAVES; ++i) L += __builtin_amdgcn_exp2f(ml[i][0][r] - ms) * ml[i][1][r];
     const float f = __builtin_amdgcn_exp2f(m - ms) * (!whole ? 1.f : L == 0.f ? 0.f : 1.f / L);
-    // half of the waves hand their parts to the other half, lane to lane, so that four parts lie in LDS
+    // half of the waves hand their parts to the other half, lane to lane: that many parts lie in LDS
     constexpr int HALF = JOIN_WAVES / 2;
     float* so = sm + (w % HALF * 16 + r) * LDO + VPL * 4 * g;
     if (w >= HALF) {
@@ -676,7 +667,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // joins the chunks of a row: out = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.  A workgroup takes COLS
 // columns of one (request, head): all of them where there are rows enough to fill the chip, 32 where
 // there are few (a single long request of 16 heads over 391 chunks: 15.6 us by whole rows, one
-// workgroup a head).  The chunks' factors are worked out once, in LDS.
+// workgroup a head; 241 chunks 3.9 us by 32 columns).  The chunks' factors are worked out once, in
+// LDS, while the first outputs are on their way.
 template <typename T, int DH, int COLS>
 __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc d, int chunk, int nsplit,
                                                          const float* __restrict__ ws_o, const float* __restrict__ ws_ml) {
@@ -789,8 +781,7 @@ static void attn_launch(const imgcap_paged_attn_desc* d, const AttnPlan& p, hipS
   float* ws_o = (float*)d->ws;
   float* ws_ml = ws_o ? ws_o + (int64_t)d->B * d->H * p.nsplit * DH : nullptr;
   const int rows_kv = d->B * d->Hkv * p.gtiles, lp = log2_of(d->page);
-  // few rows: a wave to a workgroup, so that they spread over the CUs
-  const int waves = rows_kv * (int64_t)p.nsplit >= 1024 ? 4 : 1;
+  const int waves = rows_kv >= 1024 ? 4 : 1;  // few short rows: a wave to a workgroup, so that they spread over the CUs
 #define PA_(TINY, JOIN)                                                                                          \
   hipLaunchKernelGGL((paged_attn_kernel<T, DH, TINY, JOIN>),                                                     \
                      dim3(JOIN ? rows_kv : (rows_kv + waves - 1) / waves, p.nsplit),                             \

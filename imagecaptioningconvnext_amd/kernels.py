@@ -666,8 +666,8 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
     (new[b] < 0: its pages go back).  ``table`` [B, width] int32 gets the new pages' ids, which come
     from the end of the stack ``free`` [pool] int32 holding ``count`` [1] int32 of them; the number
     left goes to ``count_out`` (default: count itself).  ``page``, tokens a page, is a power of two up to
-    1024 (1: slots are pages, and rows that stem from one row may share them).  ``tokens`` is the step's capacity, at least
-    the sum of new.  Returns (lens [B] int32, starts [B + 1] int32, slots [tokens] int64, rows
+    1024 (1: slots are pages, and rows that stem from one row may share them).  ``tokens`` is the
+    step's capacity, at least the sum of new.  Returns (lens [B] int32, starts [B + 1] int32, slots [tokens] int64, rows
     [tokens] int32, positions [tokens] int64, waits [B] int32); pass it back as ``out`` to have it
     filled again (a captured graph's outputs); ``past`` may be its lens, so that a loop's lengths go on
     in place.  A request that does not fit -- lengths past the table,

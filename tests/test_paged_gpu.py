@@ -562,3 +562,23 @@ def test_plan_outputs_at_odd_places(hip_device):
         _plan_check(case, dev, out=tuple(b[1:-2] for b in bufs))
         for b in bufs:
             assert b[0] == 55 and bool((b[-2:] == 55).all())
+
+
+@pytest.mark.parametrize("B,page,hi,add,width", [(3, 64, 50, 700000, 0), (2, 1, 9, 5, (1 << 20) + 3), (4500, 2, 9, 3, 0),
+                                                 (1100, 1, 9, 30, 0)])
+def test_plan_large(hip_device, B, page, hi, add, width):
+    """More than a million tokens, a table wider than a million pages, more requests than the token pass
+    keeps in LDS: the forms with 64-bit sums and a second launch."""
+    past, new, table, free, count, page, tokens = _plan_case(B, page, hi, add, 25, ended=0.2, extra=5)
+    if width:
+        table = torch.cat([table, torch.full((B, width - table.shape[1]), -1)], 1)
+    K, i32 = _k(), dict(dtype=torch.int32, device=hip_device)
+    short = [r[:max(1, (hi + add) // page + 2)] for r in table.tolist()]
+    want, wtable, wfree, wleft = _plan_ref(past.tolist(), new.tolist(), short, free.tolist(), count, page, tokens)
+    t, f, c = table.to(**i32), free.to(**i32), torch.tensor([count], **i32)
+    got = K.paged_plan(past.to(**i32), new.to(**i32), t, f, c, page, tokens)
+    for x, w in zip(got, want):
+        assert x.tolist() == w
+    n = len(short[0])
+    assert t[:, :n].tolist() == [r[:n] for r in wtable] and bool((t[:, n:] == -1).all())
+    assert f.tolist() == wfree and c.item() == wleft
