@@ -481,7 +481,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   asm volatile("" : "+v"(pages.now[0]), "+s"(len));  // loaded side by side, not one after the other
   const int n = min(max(len, 0), d.max_len);
   if (split > 0 && t0 >= n) return;
-  const int t1 = min(n, t0 + chunk);
+  const int t1 = t0 + min(chunk, n - t0);  // t0 + chunk may pass 32 bits
   const T* kb = (const T*)d.k + (long)kvh * d.k_head;
   const T* vb = (const T*)d.v + (long)kvh * d.v_head;
   const float c = d.scale * 1.44269504088896341f;
@@ -679,7 +679,7 @@ __global__ __launch_bounds__(256) void paged_join_kernel(imgcap_paged_attn_desc 
   const int row = blockIdx.x / (DH / COLS), c0 = blockIdx.x % (DH / COLS) * COLS, b = row / d.H, h = row % d.H;
   const int n = min(max(d.lens[b], 0), d.max_len);
   if (n <= chunk) return;
-  const int ns = (n + chunk - 1) / chunk, w = threadIdx.x >> 6;
+  const int ns = (n - 1) / chunk + 1, w = threadIdx.x >> 6;  // n + chunk may pass 32 bits
   const float* ml = ws_ml + (long)row * nsplit * 2;
   const int c4 = threadIdx.x % C4, pt = threadIdx.x / C4;
   const float* oo = ws_o + (long)row * nsplit * DH + c0 + 4 * c4;
@@ -757,7 +757,7 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
 //  - Else chunks of 512 tokens, shorter (to 128) where that leaves CUs without one, longer where it
 //    leaves more than 4096 (48 requests of up to 20011 tokens, 8 kv heads of 128: 402 us with 2048
 //    workgroups, 393 with 4096; 432 with 1024).
-struct AttnPlan { int gtiles, chunk, nsplit; bool join; };
+struct AttnPlan { int gtiles, chunk, nsplit; bool join; };  // nsplit: 1 .. MAX_SPLIT
 static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
   AttnPlan p;
   p.gtiles = (d->H / d->Hkv + 15) / 16;
@@ -769,7 +769,7 @@ static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
   if (chunk < (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT) chunk = (d->max_len + MAX_SPLIT - 1) / MAX_SPLIT;
   if (chunk > d->max_len || d->max_len <= (rows >= 256 ? 1024 : 512)) chunk = d->max_len;
   p.chunk = (int)((chunk + 31) / 32 * 32);
-  p.nsplit = (d->max_len + p.chunk - 1) / p.chunk;
+  p.nsplit = (d->max_len - 1) / p.chunk + 1;  // max_len + chunk may pass 32 bits
   return p;
 }
 static int64_t attn_ws(const imgcap_paged_attn_desc* d, const AttnPlan& p) {
@@ -876,8 +876,7 @@ extern "C" int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* str
   if (int rc = attn_check(d)) return rc;
   if (d->B == 0) return 0;
   const AttnPlan p = attn_plan(d);
-  IMGCAP_REQUIRE((int64_t)d->B * d->Hkv * p.gtiles < (1ll << 31) && (int64_t)d->B * d->H < (1ll << 31) &&
-                     p.nsplit <= 65535,
+  IMGCAP_REQUIRE((int64_t)d->B * d->Hkv * p.gtiles < (1ll << 31) && (int64_t)d->B * d->H < (1ll << 31),
                  "imgcap_paged_attention: too many rows");
   const int64_t need = attn_ws(d, p);
   if (need > 0 && !(d->ws && aligned16(d->ws) && d->ws_bytes >= need))

@@ -54,6 +54,22 @@ def test_attention_needs_its_workspace():
     assert _abi.lib().imgcap_paged_attention(ctypes.byref(empty), None) == 0
 
 
+MOST = (1 << 31) - 65536  # positions of the widest table
+
+
+@pytest.mark.parametrize("max_len", [MOST, MOST - 1, MOST - 31, 2130706432, 1900000000, 1200000000, 1 << 30, 600000, 4097])
+@pytest.mark.parametrize("B", [1, 2, 17, 128, 1000, 2047])
+def test_attention_workspace_of_long_lengths(B, max_len):
+    """Lengths near the bound, whose sum with a part's length passes 32 bits: the workspace is a maximum, a
+    sum and an output per part, of 2 to 1024 parts, where the rows alone are fewer than half of the
+    4096 workgroups that the length is cut for."""
+    d, need = _attn(B=B, H=1, Hkv=1, page=1024, width=(MOST + 1023) // 1024, max_len=max_len), ctypes.c_int64(0)
+    assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == 0
+    parts, rest = divmod(need.value, B * (64 + 2) * 4)
+    assert rest == 0 and 2 <= parts <= 1024
+    assert _abi.lib().imgcap_paged_attention(ctypes.byref(d), None) == _abi.IMGCAP_EWORKSPACE
+
+
 @pytest.mark.parametrize("kw,why", [
     (dict(dtype=3), "dtype"), (dict(dh=60), "16-byte"), (dict(heads=0), "16-byte"), (dict(n=-1), "16-byte"),
     (dict(page=24), "power of two"), (dict(pages=0), "power of two"), (dict(k=None), "NULL"), (dict(slots=None), "NULL"),

@@ -222,6 +222,45 @@ def test_attention_far_offsets(hip_device, page):
     assert bool(((got.cpu().double() - out).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("B", [1, 150, 2500])
+def test_attention_widest_table(hip_device, dtype, B):
+    """A table of the most positions there can be (2^31 - 65536), with ordinary requests in it: lengths of
+    parts, their number and the places where they begin come near 2^31 (1024 parts, 27, 2)."""
+    K, dev = _k(), hip_device
+    lens = [1 + 977 * (b % 4) for b in range(B)]
+    lens[0] = 2500
+    kc, vc, table = _cache([4096], 1024, 2, 64, dtype, 30, dev)
+    wide = torch.full((1, ((1 << 31) - 65536) // 1024), -1, dtype=torch.int32, device=dev)
+    wide[:, :4] = table[:, :4]
+    q = torch.randn(B, 2, 64, generator=torch.Generator().manual_seed(31)).to(dtype).to(dev)
+    got = K.paged_attention(q, kc, vc, wide.expand(B, -1), torch.tensor(lens, dtype=torch.int32, device=dev))
+    few = sorted({0, 1, 2, 3, B // 2, B - 2, B - 1} & set(range(B)))
+    out, _, tol, _ = _reference(q[few], kc, vc, table.expand(B, -1)[few], [lens[b] for b in few], 0.125)
+    assert bool(((got[few].cpu().double() - out).abs() <= tol).all())
+
+
+def test_attention_of_the_longest_row(hip_device):
+    """2^31 - 65541 positions on three pages that come again and again and a last one, whose last
+    position alone outweighs all others, so that a part that is cut short shows.  Scores: 40 against 0, so the others weigh 2^31 e^-40 =
+    5e-9 in all, beside the output's half step and the two bf16 pieces of a weight."""
+    K, dev = _k(), hip_device
+    width = ((1 << 31) - 65536) // 1024
+    n = width * 1024 - 5
+    table = (torch.arange(width, device=dev, dtype=torch.int32) % 3)[None].clone()
+    table[0, -1] = 3
+    g = torch.Generator().manual_seed(32)
+    q = torch.randn(1, 1, 64, generator=g).to(BF).to(dev)
+    kc = torch.zeros(4, 1024, 1, 64, dtype=BF, device=dev)
+    vc = torch.randn(4, 1024, 1, 64, generator=g).to(BF).to(dev)
+    x = q[0, 0].double()
+    kc[3, (n - 1) % 1024, 0] = (320 * x / (x @ x)).to(BF)
+    kc[3, n % 1024:] = float("nan")
+    want = vc[3, (n - 1) % 1024, 0].double()
+    got = K.paged_attention(q, kc, vc, table, torch.tensor([n], dtype=torch.int32, device=dev))
+    assert bool(((got[0, 0].double() - want).abs() <= (2.0 ** -15 + HALF[BF]) * want.abs() + 1e-7).all())
+
+
 def test_attention_captured_twice_and_on_another_stream(hip_device):
     """Two captured graphs of a split length replay in turn, with eager calls between, on new inputs;
     then the same on a stream of its own."""
