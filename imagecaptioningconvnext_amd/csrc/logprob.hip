@@ -361,16 +361,18 @@ extern "C" int imgcap_token_logprobs(const imgcap_logprob_desc* d, void* stream)
   // Few rows: 1024 threads each, for latency (5 x 9490 6.1 us).  More than 512: 256 threads for rows that
   // these hold in registers or nearly (3264 x 9490 22 us, 30 with 512), 512 beyond (1280 x 50257 fp32
   // 50.4 us, 53.4 with 256; 1000 x 131072 bf16 61, 64 with 256).
+  const int vec = d->dtype == IMGCAP_BF16 ? 8 : 4, nvec = (V + 2 * vec - 2) / vec;
+  const int tpb = n <= 512 ? 1024 : nvec <= 512 * 8 ? 256 : 512;
+  IMGCAP_REQUIRE((int64_t)n * tpb < (1ll << 32), "imgcap_token_logprobs: too many rows for a launch (2^32 threads)");
 #define LP_(T, TPB, LONG)                                                                                 \
   hipLaunchKernelGGL((token_logprobs_kernel<T, TPB, LONG>), dim3(n), dim3(TPB), 0, st, V, top,            \
                      (const T*)d->logits, (long)d->ld, d->targets, d->logp, d->entropy, d->stats, d->top_logp, d->top_ids)
 #define LP_T(T)                                                                                           \
   do {                                                                                                    \
-    const int vec = 16 / (int)sizeof(T), nvec = (V + 2 * vec - 2) / vec;                                  \
-    if (n > 512 && nvec <= 512 * 8) {                                                                     \
+    if (tpb == 256) {                                                                                     \
       if (nvec <= 256 * 8) LP_(T, 256, false);                                                            \
       else LP_(T, 256, true);                                                                             \
-    } else if (n > 512) {                                                                                 \
+    } else if (tpb == 512) {                                                                              \
       LP_(T, 512, true);                                                                                  \
     } else {                                                                                              \
       if (nvec <= 1024 * 8) LP_(T, 1024, false);                                                          \
@@ -398,7 +400,8 @@ extern "C" int imgcap_token_logprobs_bwd(const imgcap_logprob_desc* d, void* str
 #define LPB_(T)                                                                                                     \
   do {                                                                                                              \
     const int vec = 16 / (int)sizeof(T), blocks = ((V + 2 * vec - 2) / vec + 1023) / 1024;                          \
-    IMGCAP_REQUIRE((int64_t)n * blocks < (1ll << 31), "imgcap_token_logprobs_bwd: too many rows");                  \
+    IMGCAP_REQUIRE((int64_t)n * blocks < (1ll << 24),                                                               \
+                   "imgcap_token_logprobs_bwd: too many rows for a launch (2^32 threads)");                         \
     hipLaunchKernelGGL(token_logprobs_bwd_kernel<T>, dim3((unsigned)n * blocks), dim3(256), 0, st, V, blocks,       \
                        (const T*)d->logits, (long)d->ld, d->targets, d->stats, d->entropy, d->dlogp,                \
                        d->dentropy, (T*)d->dlogits, (long)d->ldd,                                                   \

@@ -743,6 +743,8 @@ static int attn_check(const imgcap_paged_attn_desc* d) {
   bool whole = aligned16(d->q) && aligned16(d->k) && aligned16(d->v);
   for (const auto& m : dims) whole = whole && (m.size <= 1 || m.stride % vec == 0);  // no stride where there is one of it
   IMGCAP_REQUIRE(whole, "paged attention: q, k and v must be 16-byte aligned with strides of whole 16 bytes");
+  // below this, rows times max_len stay within 63 bits; a launch takes fewer still (attn_fits)
+  IMGCAP_REQUIRE((int64_t)d->B * d->Hkv * ((d->H / d->Hkv + 15) / 16) < (1ll << 26), "paged attention: too many rows");
   return 0;
 }
 
@@ -771,6 +773,12 @@ static AttnPlan attn_plan(const imgcap_paged_attn_desc* d) {
   p.chunk = (int)((chunk + 31) / 32 * 32);
   p.nsplit = (d->max_len - 1) / p.chunk + 1;  // max_len + chunk may pass 32 bits
   return p;
+}
+// A launch has fewer than 2^32 threads: 256 a row of workgroups, 64 a row that a wave has to itself
+// (attn_check).  The join has no more of them: a length is split for fewer than 4096 rows only.
+static int attn_fits(const imgcap_paged_attn_desc* d, const AttnPlan& p) {
+  IMGCAP_REQUIRE(!p.join || (int64_t)d->B * d->Hkv * p.gtiles < (1ll << 24), "paged attention: too many rows");
+  return 0;
 }
 static int64_t attn_ws(const imgcap_paged_attn_desc* d, const AttnPlan& p) {
   return p.nsplit > 1 ? (int64_t)d->B * d->H * p.nsplit * (d->dh + 2) * 4 : 0;
@@ -868,7 +876,9 @@ extern "C" int imgcap_paged_write(const imgcap_paged_write_desc* d, void* stream
 extern "C" int imgcap_paged_attention_ws(const imgcap_paged_attn_desc* d, int64_t* bytes) {
   if (int rc = attn_check(d)) return rc;
   IMGCAP_REQUIRE(bytes != nullptr, "imgcap_paged_attention_ws: bytes NULL");
-  *bytes = attn_ws(d, attn_plan(d));
+  const AttnPlan p = attn_plan(d);
+  if (int rc = attn_fits(d, p)) return rc;
+  *bytes = attn_ws(d, p);
   return 0;
 }
 
@@ -876,8 +886,7 @@ extern "C" int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* str
   if (int rc = attn_check(d)) return rc;
   if (d->B == 0) return 0;
   const AttnPlan p = attn_plan(d);
-  IMGCAP_REQUIRE((int64_t)d->B * d->Hkv * p.gtiles < (1ll << 31) && (int64_t)d->B * d->H < (1ll << 31),
-                 "imgcap_paged_attention: too many rows");
+  if (int rc = attn_fits(d, p)) return rc;
   const int64_t need = attn_ws(d, p);
   if (need > 0 && !(d->ws && aligned16(d->ws) && d->ws_bytes >= need))
     return fail(IMGCAP_EWORKSPACE, "imgcap_paged_attention: " + std::to_string(need) +

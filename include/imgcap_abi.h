@@ -567,6 +567,8 @@ int imgcap_paged_write(const imgcap_paged_write_desc* d, void* stream);
  * a position (or whose every score is -inf) gets 0 and lse -inf.  lse (optional): natural log-sum-exp
  * of the scaled scores, [B, H] contiguous.  q, k, v 16-byte aligned with strides of whole 16 bytes.
  * max_len bounds the lengths on the host side: the launch is cut for it, and longer rows end there.
+ * Fewer than 2^24 rows (request, kv head, 16 of its query heads), or 2^26 where max_len is at most 64
+ * (fp32: 32).
  * ws: imgcap_paged_attention_ws bytes, 16-byte aligned, the call's own until it has run. */
 typedef struct imgcap_paged_attn_desc {
   int32_t dtype, B, H, Hkv, dh, page, pages, width, max_len;
@@ -594,7 +596,9 @@ int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream);
  * have no weight; a row of them alone gives logp -inf and entropy 0.
  * imgcap_token_logprobs_bwd: dlogits[n, V] (pitch ldd, written; in place of the logits if the pitches
  * agree) from dlogp[n] and dentropy[n] (either may be NULL = 0) and the forward's stats and entropy; a
- * row whose target is outside [0, V) has none from dlogp.  The alternatives are not differentiated. */
+ * row whose target is outside [0, V) has none from dlogp.  The alternatives are not differentiated.
+ * Rows of one call: fewer than 2^23 forward, 2^24 up to 32761 bf16 or 16381 fp32 words; backward fewer
+ * than 2^24 pieces of 8185 bf16 or 4093 fp32 words. */
 typedef struct imgcap_logprob_desc {
   int32_t dtype, n, V, top;
   int64_t ld, ldd;

@@ -70,6 +70,38 @@ def test_attention_workspace_of_long_lengths(B, max_len):
     assert _abi.lib().imgcap_paged_attention(ctypes.byref(d), None) == _abi.IMGCAP_EWORKSPACE
 
 
+@pytest.mark.parametrize("kw", [
+    dict(B=1 << 24, H=1, Hkv=1, max_len=33, dtype=_abi.F32), dict(B=1 << 24, H=1, Hkv=1, width=5, max_len=65),
+    dict(B=1 << 21, H=8, Hkv=8, width=64, max_len=1000), dict(B=1 << 22, H=34, Hkv=2, width=5, max_len=65),
+    dict(B=1 << 26, H=1, Hkv=1), dict(B=1 << 30, H=1 << 30, Hkv=1 << 30), dict(B=(1 << 31) - 1, H=(1 << 31) - 1, Hkv=1),
+])
+def test_attention_refuses_more_rows_than_a_launch_takes(kw):
+    """A launch has fewer than 2^32 threads; row counts whose products pass 63 bits with the length."""
+    d, need = _attn(**kw), ctypes.c_int64(-1)
+    assert _abi.lib().imgcap_paged_attention(ctypes.byref(d), None) == -1
+    assert "too many rows" in _said()
+    assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == -1
+    assert need.value == -1
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n=1 << 24), dict(n=(1 << 31) - 1), dict(n=1 << 23, V=40000, ld=40000), dict(n=1 << 24, V=32761, ld=32761),
+    dict(n=1 << 23, V=16390, ld=16390, dtype=_abi.F32),
+])
+def test_logprobs_refuse_more_rows_than_a_launch_takes(kw):
+    assert _abi.lib().imgcap_token_logprobs(ctypes.byref(_logprobs(**kw)), None) == -1
+    assert "too many rows" in _said()
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n=1 << 24), dict(n=1 << 23, V=9490, ldd=9490, ld=9490), dict(n=1 << 20, V=131072, ld=131072, ldd=131072),
+    dict(n=1 << 23, V=5000, ld=5000, ldd=5000, dtype=_abi.F32),
+])
+def test_logprobs_bwd_refuses_more_rows_than_a_launch_takes(kw):
+    assert _abi.lib().imgcap_token_logprobs_bwd(ctypes.byref(_logprobs(**kw)), None) == -1
+    assert "too many rows" in _said()
+
+
 @pytest.mark.parametrize("kw,why", [
     (dict(dtype=3), "dtype"), (dict(dh=60), "16-byte"), (dict(heads=0), "16-byte"), (dict(n=-1), "16-byte"),
     (dict(page=24), "power of two"), (dict(pages=0), "power of two"), (dict(k=None), "NULL"), (dict(slots=None), "NULL"),
