@@ -680,8 +680,8 @@ def paged_plan(past, new, table, free, count, page, tokens, *, count_out=None, o
         _mixed(name, past, new, table, free, count, count_out)
     B, pool = past.numel(), free.numel()
     table_row, width = _int_rows(name, "table", table, B)
-    if not (0 < page <= 1024 and 0 <= tokens < 1 << 31 and pool < 1 << 31):  # the C side's integers have 32 bits
-        raise ValueError(f"paged_plan: page {page}, tokens {tokens} or pool {pool} out of range")
+    if not (0 < page <= 1024 and tokens >= 0) or (B | width | pool | tokens) >> 31:  # the C side's integers have 32 bits
+        raise ValueError(f"paged_plan: page {page}, tokens {tokens}, pool {pool}, {B} rows or width {width} out of range")
     i32, i64, rows_shape = torch.int32, torch.int64, (B,)
     if not (past.dtype is new.dtype is free.dtype is count.dtype is count_out.dtype is i32 and past.shape == rows_shape
             and new.shape == rows_shape and count.numel() == 1 and count_out.numel() == 1 and free.dim() == 1
@@ -740,6 +740,8 @@ def paged_write(k, v, k_cache, v_cache, slots):
         _want(name, "slots", slots, torch.int64, (n,))
     if n == 0:
         return
+    if (n | heads | dh | page | pages) >> 31:  # the C side's integers have 32 bits
+        raise ValueError(f"paged_write: {n} rows or a cache of {tuple(shape)} out of range")
     d = _abi.PagedWriteDesc(dt(k), n, heads, dh, page, pages, ks[0], ks[1], vs[0], vs[1], kc[0], kc[1], kc[2], vc[0],
                             vc[1], vc[2], k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                             slots.data_ptr())
@@ -784,6 +786,9 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
         _want(name, "lse", lse, torch.float32, (B, H))
     if B == 0:
         return out
+    if (B | H | hkv | page | pages | width) >> 31:  # the C side's integers have 32 bits
+        raise ValueError(f"paged_attention: {B} rows, {H} heads, {width} pages a row or a cache of "
+                         f"{tuple(k_cache.shape)} out of range")
     if max_len is None:
         max_len = width * page
     elif not 0 < max_len <= width * page:
@@ -811,6 +816,8 @@ def _logit_rows(name, logits, V):
     V = cols if V is None else V
     if not 0 < V <= cols:
         raise ValueError(f"{name}: V must be in 1 .. {cols}")
+    if (n | V) >> 31:  # the C side's integers have 32 bits
+        raise ValueError(f"{name}: {n} rows of {V} words out of range")
     return n, V, (logits.stride(0) if n > 1 else cols)
 
 

@@ -180,3 +180,42 @@ def test_wrappers_refuse_cpu_tensors():
                  lambda: K.token_logprobs_bwd(x[0], None, x[0], x[0, 0])):
         with pytest.raises(RuntimeError, match="GPU"):
             call()
+
+
+FAR = (1 << 32) + 1  # one, in 32 bits
+
+
+def _calls_past_32_bits():
+    def rows(n, *shape, dtype=torch.float32):  # n of them, all the same
+        return torch.zeros(1, *shape, dtype=dtype).expand(n, *(-1 for _ in shape))
+
+    i32 = dict(dtype=torch.int32)
+    q, c, t, i = torch.zeros(1, 1, 64), torch.zeros(2, 16, 1, 64), torch.zeros(1, 4, **i32), torch.zeros(1, **i32)
+
+    def meta(*shape, dtype=torch.int32):  # no memory behind it
+        return torch.empty(*shape, dtype=dtype, device="meta")
+
+    return {
+        "attention, pages": lambda: K.paged_attention(q, rows(FAR, 16, 1, 64), rows(FAR, 16, 1, 64), t, i, out=q),
+        "attention, heads": lambda: K.paged_attention(rows(FAR, 64)[None], c, c, t, i, out=rows(FAR, 64)[None]),
+        "attention, width": lambda: K.paged_attention(q, c, c, meta(1, FAR), i, max_len=5, out=q),
+        "write, pages": lambda: K.paged_write(q, q, rows(FAR, 16, 1, 64), rows(FAR, 16, 1, 64), i.long()),
+        "write, heads": lambda: K.paged_write(*[rows(FAR, 64)[None]] * 2, *[c.expand(2, 16, FAR, 64)] * 2, i.long()),
+        "plan, pool": lambda: K.paged_plan(i, i, t, meta(FAR), i, 16, 2),
+        "plan, rows": lambda: K.paged_plan(meta(FAR), meta(FAR), meta(FAR, 4), i, i, 16, 2),
+        "plan, width": lambda: K.paged_plan(i, i, meta(1, FAR), i, i, 16, 2),
+        "logprobs, rows": lambda: K.token_logprobs(rows(FAR, 4)),
+        "logprobs, words": lambda: K.token_logprobs(meta(1, FAR, dtype=torch.float32)),
+    }
+
+
+@pytest.mark.parametrize("what", list(_calls_past_32_bits()))
+def test_wrappers_refuse_counts_past_32_bits(monkeypatch, what):
+    """Counts whose low 32 bits are an ordinary number never reach the descriptors, which would keep those."""
+    went = []
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(torch.Tensor, "new_empty", lambda t, *a, **k: torch.empty(0))
+    monkeypatch.setattr(K, "_run_on", lambda *a: went.append(a) or 0)
+    with pytest.raises(ValueError, match="out of range"):
+        _calls_past_32_bits()[what]()
+    assert not went
