@@ -118,9 +118,11 @@ class TransformerDecoder(nn.Module):
 
     def logProbs(self, encoder_out, encoded_captions, caption_lengths, tgt_key_padding_mask=None, top=0):
         """Log-probabilities of the captions' own tokens, teacher forced: (logp [B, L], entropy [B, L] in
-        nats, top_logp [B, L, top], top_ids [B, L, top]); position l predicts token l + 1, positions past
-        a caption's last target have logp 0.  One pass over the logits, which are never held in fp32.
-        Differentiable in logp and entropy (scoring, policy-gradient training on sampled captions)."""
+        nats, top_logp [B, L, top], top_ids [B, L, top]); position l predicts token l + 1.  Positions past
+        a caption's last target have logp 0, without a gradient; entropy and alternatives there are those
+        of the padded position, so a mean over the captions' own positions masks them out.  One pass over
+        the logits, which are never held in fp32.  Differentiable in logp and in every position's entropy
+        (scoring, policy-gradient training on sampled captions)."""
         eng = self.engine()
         key_ids, pad_id = self._padding(encoded_captions, tgt_key_padding_mask)
         return _TransformerLogProbs.apply(eng, encoder_out, encoded_captions, caption_lengths, key_ids, pad_id, top,

@@ -218,7 +218,7 @@ class TransformerEngine:
         """Of a forward(loss=False): log-probability of every target token, entropy of every position
         and its ``top`` best alternatives, (logp [B, L], entropy [B, L], top_logp [B, L, top], top_ids
         [B, L, top]) in one pass over the logits (imgcap_token_logprobs).  Positions past a caption's
-        last target have logp 0; their entropy is that of the row as it stands."""
+        last target have logp 0; their entropy and alternatives are those of the row as it stands."""
         B, L, V = s["B"], s["L"], self.V
         logits = torch.empty(B * L, self.Vpad, device=s["xL"].device, dtype=self.ct)
         K.gemm(s["xL"], self.fp.w("fc_out.weight"), trans_b=True, bias=self.fp.f32("fc_out.bias"), out=logits, N=V)
@@ -228,13 +228,13 @@ class TransformerEngine:
 
     def logprobs_backward(self, s, dlogp=None, dentropy=None, gbuf=None, want_denc=False):
         """Gradients of every parameter (and, ``want_denc``, of the encoder's output: s["denc"]) from
-        those of logprobs' logp and entropy [B, L] (either may be None) into ``gbuf``; positions past a
-        caption's last target have none."""
+        those of logprobs' logp and entropy [B, L] (either may be None) into ``gbuf``.  A position past a
+        caption's last target has none from its logp, which is 0 there; its entropy has its own."""
         logits, stats, entropy = s["logprobs"]
         V = self.V
 
-        def rows(g):
-            return None if g is None else torch.where(s["tmask"], g.float(), 0.0).reshape(-1)
+        def rows(g):  # a sum's or a mean's gradient comes expanded
+            return None if g is None else g.float().reshape(-1).contiguous()
 
         dl = torch.empty_like(logits)
         if self.Vpad > V:

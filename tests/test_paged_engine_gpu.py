@@ -185,6 +185,37 @@ def test_log_probs_and_gradients(hip_device, masked):
         assert _rel(params[name].grad, q.grad) < 1e-4, name
 
 
+@pytest.mark.parametrize("loss", ["mean", "weighted"])
+@pytest.mark.parametrize("masked", [False, True])
+def test_entropy_gradient_is_that_of_every_position(hip_device, masked, loss):
+    """The entropy of the positions past a caption's last target has a value, so it has a gradient too: a
+    loss over all positions (a mean, whose gradient comes expanded, and one of its own weights) against
+    autograd through the oracle in 64 bits.  logp there is 0 whatever the parameters are."""
+    dec, p = _model(hip_device)
+    B, L = 4, 14
+    caps, lens = make_captions(B, L, [14, 9, 3, 12], CFG["V"], 13)
+    enc = make_features((B, 7, 7, CFG["E"]), 14)
+    pad = (caps == 0) if masked else torch.zeros_like(caps, dtype=torch.bool)
+    h = torch.randn(B, L, generator=torch.Generator().manual_seed(18))
+    live = torch.arange(L) < lens - 1
+
+    def value(logp, ent, w):
+        return logp.sum() / 20 + ent.mean() if loss == "mean" else (logp * w + ent * w).sum()
+
+    x = enc.to(hip_device).requires_grad_(True)
+    logp, ent, _, _ = dec.logProbs(x, caps.to(hip_device), lens.to(hip_device), pad.to(hip_device) if masked else None)
+    value(logp, ent, h.to(hip_device)).backward()
+    pr = {k: v.clone().requires_grad_(True) for k, v in p.items()}
+    ex = enc.double().requires_grad_(True)
+    logq = torch.log_softmax(_oracle(pr, ex, caps, lens, pad), -1)
+    wlogp = torch.where(live, logq.gather(-1, torch.where(live, torch.roll(caps, -1, 1), 0)[..., None])[..., 0], 0.0)
+    value(wlogp, -(logq.exp() * logq).sum(-1), h.double()).backward()
+    assert _rel(x.grad, ex.grad) < 1e-4
+    params = dict(dec.named_parameters())
+    for name, q in pr.items():
+        assert _rel(params[name].grad, q.grad) < 1e-4, name
+
+
 def test_log_probs_are_those_of_the_predictions(hip_device):
     """bf16 at the captions' own width: the fused pass against log_softmax of the same bf16 logits."""
     dec, _ = _model(hip_device, torch.bfloat16)
