@@ -223,7 +223,7 @@ class TransformerEngine:
         logits = torch.empty(B * L, self.Vpad, device=s["xL"].device, dtype=self.ct)
         K.gemm(s["xL"], self.fp.w("fc_out.weight"), trans_b=True, bias=self.fp.f32("fc_out.bias"), out=logits, N=V)
         logp, entropy, stats, top_logp, top_ids = K.token_logprobs(logits, s["targets"], V, top=top)
-        s["logprobs"] = (logits, stats, entropy)
+        s["logprobs"] = (logits, stats, entropy.clone())  # the caller may change the one that it gets
         return logp.view(B, L), entropy.view(B, L), top_logp.view(B, L, top), top_ids.view(B, L, top)
 
     def logprobs_backward(self, s, dlogp=None, dentropy=None, gbuf=None, want_denc=False):

@@ -216,6 +216,28 @@ def test_entropy_gradient_is_that_of_every_position(hip_device, masked, loss):
         assert _rel(params[name].grad, q.grad) < 1e-4, name
 
 
+def test_outputs_changed_by_the_caller_leave_the_backward_alone(hip_device):
+    """The tensors that logprobs returns are the caller's: the backward does not read them again."""
+    dec, _ = _model(hip_device)
+    B, L = 3, 12
+    caps, lens = make_captions(B, L, [12, 5, 8], CFG["V"], 19)
+    enc = make_features((B, 7, 7, CFG["E"]), 20).to(hip_device)
+    eng = dec.engine()
+    gen = torch.Generator().manual_seed(21)
+    g, h = (torch.randn(B, L, generator=gen).to(hip_device) for _ in range(2))
+    grads = []
+    for change in (False, True):
+        s = eng.forward(enc, caps.to(hip_device), lens.to(hip_device), loss=False)
+        out = eng.logprobs(s, 3)
+        if change:
+            for t in out:
+                t.fill_(7)
+        buf = torch.empty_like(eng.fp.grad)
+        eng.logprobs_backward(s, g, h, gbuf=buf)
+        grads.append(buf)
+    assert torch.equal(*grads)
+
+
 def test_log_probs_are_those_of_the_predictions(hip_device):
     """bf16 at the captions' own width: the fused pass against log_softmax of the same bf16 logits."""
     dec, _ = _model(hip_device, torch.bfloat16)
