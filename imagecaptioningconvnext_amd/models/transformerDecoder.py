@@ -60,7 +60,7 @@ class _TransformerLogProbs(torch.autograd.Function):
         s = engine.forward(encoder_out, caps, caplens, key_ids=key_ids, pad_id=pad_id, loss=False)
         ctx.engine, ctx.s = engine, s
         ctx.enc_shape, ctx.enc_dtype = encoder_out.shape, encoder_out.dtype
-        logp, entropy, top_logp, top_ids = engine.logprobs(s, top)
+        logp, entropy, top_logp, top_ids = engine.logprob_rows(s, top)  # no views: the caller may change them in place
         ctx.mark_non_differentiable(top_logp, top_ids)
         return logp, entropy, top_logp, top_ids
 
@@ -125,8 +125,9 @@ class TransformerDecoder(nn.Module):
         (scoring, policy-gradient training on sampled captions)."""
         eng = self.engine()
         key_ids, pad_id = self._padding(encoded_captions, tgt_key_padding_mask)
-        return _TransformerLogProbs.apply(eng, encoder_out, encoded_captions, caption_lengths, key_ids, pad_id, top,
+        rows = _TransformerLogProbs.apply(eng, encoder_out, encoded_captions, caption_lengths, key_ids, pad_id, top,
                                           *eng.fp.params.values())
+        return tuple(r.view(*encoded_captions.shape, *r.shape[1:]) for r in rows)
 
     def forwardWithTeacherForcing(self, encoder_out, encoded_captions, caption_lengths, tgt_key_padding_mask):
         eng = self.engine()

@@ -219,16 +219,22 @@ class TransformerEngine:
         and its ``top`` best alternatives, (logp [B, L], entropy [B, L], top_logp [B, L, top], top_ids
         [B, L, top]) in one pass over the logits (imgcap_token_logprobs).  Positions past a caption's
         last target have logp 0; their entropy and alternatives are those of the row as it stands."""
-        B, L, V = s["B"], s["L"], self.V
-        logits = torch.empty(B * L, self.Vpad, device=s["xL"].device, dtype=self.ct)
+        B, L = s["B"], s["L"]
+        logp, entropy, top_logp, top_ids = self.logprob_rows(s, top)
+        return logp.view(B, L), entropy.view(B, L), top_logp.view(B, L, top), top_ids.view(B, L, top)
+
+    def logprob_rows(self, s, top=0):
+        """logprobs by rows of the logits: [B * L] and [B * L, top], tensors of their own (no views)."""
+        V = self.V
+        logits = torch.empty(s["B"] * s["L"], self.Vpad, device=s["xL"].device, dtype=self.ct)
         K.gemm(s["xL"], self.fp.w("fc_out.weight"), trans_b=True, bias=self.fp.f32("fc_out.bias"), out=logits, N=V)
         logp, entropy, stats, top_logp, top_ids = K.token_logprobs(logits, s["targets"], V, top=top)
         s["logprobs"] = (logits, stats, entropy.clone())  # the caller may change the one that it gets
-        return logp.view(B, L), entropy.view(B, L), top_logp.view(B, L, top), top_ids.view(B, L, top)
+        return logp, entropy, top_logp, top_ids
 
     def logprobs_backward(self, s, dlogp=None, dentropy=None, gbuf=None, want_denc=False):
         """Gradients of every parameter (and, ``want_denc``, of the encoder's output: s["denc"]) from
-        those of logprobs' logp and entropy [B, L] (either may be None) into ``gbuf``.  A position past a
+        those of logprobs' logp and entropy [B, L] (or [B * L]; either may be None) into ``gbuf``.  A position past a
         caption's last target has none from its logp, which is 0 there; its entropy has its own."""
         logits, stats, entropy = s["logprobs"]
         V = self.V

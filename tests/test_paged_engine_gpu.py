@@ -238,6 +238,34 @@ def test_outputs_changed_by_the_caller_leave_the_backward_alone(hip_device):
     assert torch.equal(*grads)
 
 
+def test_log_probs_changed_in_place(hip_device):
+    """Padding masked out in place, as logits and losses usually are: the same gradients as out of place,
+    and a second backward through the same graph gives them again."""
+    dec, _ = _model(hip_device)
+    B, L = 3, 12
+    caps, lens = make_captions(B, L, [12, 5, 8], CFG["V"], 19)
+    enc = make_features((B, 7, 7, CFG["E"]), 20).to(hip_device)
+    dead = (torch.arange(L) >= lens - 1).to(hip_device)
+    params = list(dec.parameters())
+
+    def grads(inplace, times=1):
+        logp, ent, tl, ti = dec.logProbs(enc, caps.to(hip_device), lens.to(hip_device), top=2)
+        assert logp.shape == ent.shape == (B, L) and tl.shape == ti.shape == (B, L, 2) and not tl.requires_grad
+        if inplace:
+            ent[dead] = 0
+            logp.mul_(2)
+            tl[dead] = -1
+        else:
+            ent, logp = torch.where(dead, 0.0, ent), 2 * logp
+        for i in range(times):
+            g = torch.autograd.grad(logp.sum() + ent.sum(), params, retain_graph=i + 1 < times)
+        return g
+
+    want = grads(False)
+    for got in (grads(True), grads(True, 2)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_log_probs_are_those_of_the_predictions(hip_device):
     """bf16 at the captions' own width: the fused pass against log_softmax of the same bf16 logits."""
     dec, _ = _model(hip_device, torch.bfloat16)
