@@ -453,6 +453,10 @@ DEV uint32_t pack_bf16(float a, float b) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (bf16)a) | ((uint32_t)__builtin_bit_cast(uint16_t, (bf16)b) << 16);
 }
 
+// what is left of weight a beside its top bits, at least 2^-24 of it, the smallest normal number where that
+// is none; 0 for a weight of 0, so that its value, however large, adds nothing
+DEV float weight_rest(float a, float top) { return fmaxf(fmaxf(a - top, a * 0x1p-24f), fminf(a, 0x1p-126f)); }
+
 // JOIN: the workgroup's waves share a chunk (blockIdx.x the row, blockIdx.y the chunk), 32 tokens each
 // in turn, and put their parts together in LDS.  Else each wave has a short row to itself, the waves of
 // a group consecutive rows (kv heads of the same tokens, which lie side by side in memory), and
@@ -557,16 +561,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         }
       if constexpr (sizeof(T) == 2) {
         // the weights go in as their top bf16 bits and the remainder in bf16: 15 bits and more of them,
-        // so the output carries little but its own rounding.  Both pieces are kept positive (the
-        // remainder at least 1e-30, nothing beside a weight that counts): an infinite value times a
-        // zero or negative remainder would turn the infinity into NaN.
+        // so the output carries little but its own rounding.  Both pieces of a weight above 0 are kept
+        // positive (weight_rest): an infinite value times a zero or negative remainder would turn the
+        // infinity into NaN.
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float a = p[e >> 1][2 * (e & 1)], bb = p[e >> 1][2 * (e & 1) + 1];
           hi[e] = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, bb), __builtin_bit_cast(uint32_t, a), 0x07060302u);
-          lo[e] = pack_bf16(fmaxf(a - __builtin_bit_cast(float, hi[e] << 16), 1e-30f),
-                            fmaxf(bb - __builtin_bit_cast(float, hi[e] & 0xffff0000u), 1e-30f));
+          lo[e] = pack_bf16(weight_rest(a, __builtin_bit_cast(float, hi[e] << 16)),
+                            weight_rest(bb, __builtin_bit_cast(float, hi[e] & 0xffff0000u)));
         }
         const bf16x8 ph = __builtin_bit_cast(bf16x8, make_uint4(hi[0], hi[1], hi[2], hi[3]));
         const bf16x8 pl = __builtin_bit_cast(bf16x8, make_uint4(lo[0], lo[1], lo[2], lo[3]));

@@ -191,6 +191,42 @@ def test_attention_infinities_and_nan(hip_device, dtype):
     assert bool((got == 0).all()) and bool((lse == -math.inf).all())
 
 
+@pytest.mark.parametrize("dtype", [BF, F])
+@pytest.mark.parametrize("page,n", [(16, 20), (1, 20), (16, 700), (16, 3000)])
+def test_attention_weightless_positions(hip_device, dtype, page, n):
+    """Live positions of weight 0 (scores of -200 and of -inf) that hold the type's largest values add
+    nothing; one of weight e^-72 adds its share, and an infinite value is infinity at any weight above
+    0.  Scores are exact (the query is 1 in one place); taken to base 2 one of 72 is off by 4 U 104, the
+    exponential by 2^-22, two bf16 pieces of a weight by 2^-16: less than 2^-15 of sum(p |v|) in all."""
+    kc, vc, table = _cache([n] * 3, page, 1, 64, dtype, 40, hip_device)
+    at = lambda b, t: (table[b, t // page].item(), t % page, 0)  # noqa: E731
+    kc[..., 0] = torch.where(kc[..., 0].isnan(), kc[..., 0], 0)
+    kc[..., 1:] = 0
+    q = torch.zeros(3, 2, 64, dtype=dtype, device=hip_device)
+    q[..., 0] = 1
+    for b in range(3):
+        for t in (3, n - 2):
+            kc[at(b, t)][0] = -1600
+            vc[at(b, t)] = torch.finfo(dtype).max
+        kc[at(b, 7)][0] = -math.inf
+        vc[at(b, 7)] = torch.finfo(dtype).max
+    kc[at(1, 5)][0] = -576
+    vc[at(1, 5)] = 1e31
+    lens = torch.tensor([n] * 3, dtype=torch.int32, device=hip_device)
+    got = _k().paged_attention(q, kc, vc, table, lens)
+    t = torch.arange(n, device=hip_device)
+    for b in range(3):
+        k, v = (c[table[b, t // page].long(), t % page, 0].double() for c in (kc, vc))
+        p = torch.softmax(k[:, 0] / 8, 0)[:, None]
+        want, room = (p * v).sum(0), (p * v.abs()).sum(0)
+        assert bool(((got[b].double() - want).abs() <= 2.0 ** -15 * room + HALF[dtype] * want.abs()).all()), b
+    for score in (-64, -576, -680):  # weights of e^-8, e^-72 and e^-85
+        kc[at(2, 5)][0] = score
+        vc[at(2, 5)][0] = math.inf
+        got = _k().paged_attention(q, kc, vc, table, lens)
+        assert bool((got[2, :, 0] == math.inf).all()) and bool(torch.isfinite(got[2, :, 1:]).all())
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 3.0])
 def test_attention_scale(hip_device, scale):
     kc, vc, table = _cache([50, 3], 16, 1, 128, F, 9, hip_device)
