@@ -750,6 +750,10 @@ def paged_write(k, v, k_cache, v_cache, slots):
         _abi.fail("imgcap_paged_write", rc)
 
 
+# the longest length that is never split over workgroups (paged.hip attn_plan): such a call has no scratch
+_ATTN_WHOLE = 512
+
+
 def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=None, out=None, lse=None):
     """Attention of one new token per request over its pages (imgcap_paged_attention): q [B, H, head
     dim], caches [pages, page, kv heads, head dim] of any strides, table [B, width] int32, lens [B]
@@ -797,13 +801,16 @@ def paged_attention(q, k_cache, v_cache, table, lens, *, scale=None, max_len=Non
                            dh ** -0.5 if scale is None else scale, qs[0], qs[1], os_[0], os_[1], ks[0], ks[1], ks[2],
                            vs[0], vs[1], vs[2], table_row, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
                            out.data_ptr(), ptr(lse), table.data_ptr(), lens.data_ptr(), None, 0)
-    rc = _run_on(dev, "imgcap_paged_attention", d)
-    if rc == _abi.IMGCAP_EWORKSPACE:  # a split length: the parts' maxima, sums and outputs; nothing ran yet
+    ws = None
+    if max_len > _ATTN_WHOLE:  # may be split: the parts' maxima, sums and outputs
         need = ctypes.c_int64(0)
-        _abi.check("imgcap_paged_attention_ws", d, need)
-        ws = q.new_empty(need.value, dtype=torch.uint8)
-        d.ws, d.ws_bytes = ws.data_ptr(), need.value
-        rc = _run_on(dev, "imgcap_paged_attention", d)
+        rc = _abi.lib().imgcap_paged_attention_ws(d, need)
+        if rc:
+            _abi.fail("imgcap_paged_attention", rc)
+        if need.value:
+            ws = q.new_empty(need.value, dtype=torch.uint8)
+            d.ws, d.ws_bytes = ws.data_ptr(), need.value
+    rc = _run_on(dev, "imgcap_paged_attention", d)
     if rc:
         _abi.fail("imgcap_paged_attention", rc)
     return out

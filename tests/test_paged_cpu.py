@@ -219,3 +219,42 @@ def test_wrappers_refuse_counts_past_32_bits(monkeypatch, what):
     with pytest.raises(ValueError, match="out of range"):
         _calls_past_32_bits()[what]()
     assert not went
+
+
+def _attention_calls(monkeypatch, B, H, max_len):
+    """The descriptors that a paged_attention of CPU tensors would launch, and the error text before and after."""
+    seen = []
+
+    def run(dev, name, d):
+        seen.append((name, d.max_len, d.ws_bytes, bool(d.ws)))
+        return 0
+
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    monkeypatch.setattr(K, "_run_on", run)
+    width = (max_len + 15) // 16
+    q, c = torch.zeros(B, H, 64), torch.zeros(1, 16, 1, 64)
+    t, i = torch.zeros(1, width, dtype=torch.int32).expand(B, width), torch.zeros(B, dtype=torch.int32)
+    K.paged_attention(q, c, c, t, i, max_len=max_len)
+    return seen
+
+
+@pytest.mark.parametrize("B,H,max_len", [(1, 1, 513), (2, 16, 5000), (1, 3, 100000), (300, 1, 1024), (300, 1, 1025), (1, 1, 512)])
+def test_attention_is_called_once_with_its_workspace(monkeypatch, B, H, max_len):
+    """A split length is no call that fails first: one launch, with the bytes that the size query says."""
+    d, need = _attn(dtype=_abi.F32, B=B, H=H, Hkv=1, width=(max_len + 15) // 16, max_len=max_len), ctypes.c_int64(0)
+    assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == 0
+    _abi.lib().imgcap_paged_attention_ws(None, ctypes.byref(need))  # leaves an error text
+    before = _said()
+    assert _attention_calls(monkeypatch, B, H, max_len) == [("imgcap_paged_attention", max_len, need.value, need.value > 0)]
+    assert _said() == before
+
+
+@pytest.mark.parametrize("dtype", [_abi.BF16, _abi.F32])
+@pytest.mark.parametrize("B", [1, 7, 255, 256, 4096, 1 << 20])
+def test_short_lengths_take_no_workspace(dtype, B):
+    """What the wrapper takes for granted (_ATTN_WHOLE)."""
+    need = ctypes.c_int64(-1)
+    for max_len in (1, 32, 33, 64, 65, 500, K._ATTN_WHOLE):
+        d = _attn(dtype=dtype, B=B, width=64, max_len=max_len)
+        assert _abi.lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == 0
+        assert need.value == 0
