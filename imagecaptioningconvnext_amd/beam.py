@@ -117,6 +117,8 @@ def _transformer_beam(encoder, decoder, imagePath, wordMap, beamSize, max_decode
     eng = decoder.engine()
     try:
         with torch.no_grad():
+            if with_alphas:
+                eng.cross_probs = []  # decode_init refuses more positions than can be recorded
             st = eng.decode_init(encoderOut.reshape(1, -1, encoderDim).expand(k, -1, encoderDim), max_decode_len)
             num_pixels = st["P"]
             kPrevWords = torch.full((k, 1), wordMap['<start>'], dtype=torch.long, device=dev)

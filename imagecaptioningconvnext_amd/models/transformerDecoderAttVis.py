@@ -101,14 +101,15 @@ class TransformerDecoderForAttentionViz(nn.Module):
         eng = self.engine()
         from .. import kernels as K
         with torch.no_grad():
-            st = eng.decode_init(encoder_out, maxDecodeLen)
-            B, V, dev = st["B"], self.vocab_size, encoder_out.device
-            preds = torch.zeros(B, maxDecodeLen, V, device=dev, dtype=torch.float32)
-            seqs = torch.zeros(B, maxDecodeLen, device=dev, dtype=torch.int64)
-            alphas = torch.zeros(B, maxDecodeLen, st["P"], device=dev, dtype=torch.float32)
-            finished = torch.zeros(B, device=dev, dtype=torch.uint8)
-            ids = torch.full((B,), wordMap['<start>'], device=dev, dtype=torch.int64)
+            eng.cross_probs = []  # decode_init refuses more positions than can be recorded
             try:
+                st = eng.decode_init(encoder_out, maxDecodeLen)
+                B, V, dev = st["B"], self.vocab_size, encoder_out.device
+                preds = torch.zeros(B, maxDecodeLen, V, device=dev, dtype=torch.float32)
+                seqs = torch.zeros(B, maxDecodeLen, device=dev, dtype=torch.int64)
+                alphas = torch.zeros(B, maxDecodeLen, st["P"], device=dev, dtype=torch.float32)
+                finished = torch.zeros(B, device=dev, dtype=torch.uint8)
+                ids = torch.full((B,), wordMap['<start>'], device=dev, dtype=torch.int64)
                 for t in range(maxDecodeLen):
                     eng.cross_probs = []
                     logits = eng.decode_step(st, ids)

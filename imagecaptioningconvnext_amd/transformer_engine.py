@@ -276,13 +276,15 @@ class TransformerEngine:
         ``paged`` (default: beyond 64 positions, which the tile of the dense cache's attention kernel
         holds): keys and values lie in a pool of token-sized pages instead (kernels.paged_plan /
         paged_write / paged_attention), for any number of positions and pixels; keeping or reordering
-        rows moves rows of the page tables only.  Without dropout on the attention probabilities:
-        the decoder has to be in eval mode."""
+        rows moves rows of the page tables only.  Without dropout on the attention probabilities (the
+        decoder has to be in eval mode) and without a record of them (``cross_probs`` None)."""
         fp, ct, dev = self.fp, self.ct, encoder_out.device
         d = self.d
         paged = maxlen > 64 if paged is None else paged
         if maxlen > 64 and not paged:
             raise ValueError("step-wise decode: at most 64 positions (attention kernel tile)")
+        if paged and self.cross_probs is not None:
+            raise ValueError("step-wise decode: at most 64 positions where attention probabilities are recorded, and no pages")
         if paged and self.dec.training and self.dec.dropout_p > 0:
             raise ValueError("paged decode: no dropout on the attention probabilities, call eval() first")
         if paged and maxlen > self.dec.pos_encoding.pe.numel() // d:

@@ -99,3 +99,29 @@ def test_attvis_beam_search_matches_reference(hip_device, k):
     assert got.shape == t[f"beam.k{k}.alphas"].shape  # [max_decode_len, P], zero past the caption
     assert (got - t[f"beam.k{k}.alphas"]).abs().max().item() < 1e-5
     assert got[len(seq) - 1:].abs().sum().item() == 0.0
+
+
+def test_attvis_refuses_more_positions_than_it_records(hip_device, monkeypatch):
+    """More than 64 positions: greedy and beam search are refused before any product is made, and the
+    decoder is as it was."""
+    from imagecaptioningconvnext_amd import beam, kernels
+    from test_beam_gpu import _FixedEncoder
+    t, meta = _fixture()
+    dec = _decoder({**meta["beam"]["cfg"], "L": 80}, hip_device, end_bias=meta["beam"]["end_bias_added"])
+    wm = word_map(meta["beam"]["cfg"]["V"])
+    feats = t["beam.feats"].to(hip_device)
+
+    def greedy(n):
+        return dec(teacherForcing=False, encoder_out=feats, wordMap=wm, maxDecodeLen=n)
+
+    want = greedy(6)
+    made = []
+    with monkeypatch.context() as m:
+        m.setattr(kernels, "gemm", lambda *a, **k: made.append(a))
+        with pytest.raises(ValueError, match="64"):
+            greedy(65)
+        with pytest.raises(ValueError, match="64"):
+            beam.caption_image_beam_search_transformer_attention(_FixedEncoder(feats), dec, torch.zeros(3, 256, 256), wm,
+                                                                 "unused", max_decode_len=65)
+    assert not made and dec.engine().cross_probs is None
+    assert all(torch.equal(a, b) for a, b in zip(greedy(6), want))
