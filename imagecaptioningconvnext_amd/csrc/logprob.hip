@@ -4,8 +4,9 @@
 //   d x_j = g (1[j = target] - p_j) - h p_j (ln p_j + H)      for upstream g of logp, h of H
 // The forward leaves (m, log2 s) rather than their sum: x - m is exact near the maximum, so the
 // backward's p keeps full fp32 accuracy however large the logits are.
-// Logits of -inf (banned words) have weight zero and add nothing; a row of them alone gives
-// logp -inf, H 0 and no gradient.  NaN and +inf reach every output of their row.
+// Logits of -inf (banned words) have weight zero, add nothing and get no gradient, but for a target
+// among them, which keeps its g (1 - p = g); a row of them alone gives logp -inf and H 0.  NaN and +inf
+// reach every output of their row.
 #include "common.h"
 
 namespace imgcap {

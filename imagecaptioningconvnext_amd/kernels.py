@@ -861,7 +861,8 @@ def token_logprobs(logits, targets=None, V=None, *, top=0):
 def token_logprobs_bwd(logits, targets, stats, entropy, dlogp=None, dentropy=None, *, V=None, dlogits=None):
     """Gradient of the logits of token_logprobs from those of logp and entropy ([n] fp32, either may
     be None) -> dlogits [n, V] in the logits' dtype (of a given ``dlogits`` [n, >= V], which may be
-    ``logits`` itself, the columns from V on stay).  The alternatives have no gradient."""
+    ``logits`` itself, the columns from V on stay).  The alternatives have no gradient; a logit of -inf has
+    none either, but for a target among them, which keeps its dlogp."""
     name = "token_logprobs_bwd"
     dev = logits.get_device()
     for t in (targets, stats, entropy, dlogp, dentropy, dlogits):

@@ -597,6 +597,7 @@ int imgcap_paged_attention(const imgcap_paged_attn_desc* d, void* stream);
  * imgcap_token_logprobs_bwd: dlogits[n, V] (pitch ldd, written; in place of the logits if the pitches
  * agree) from dlogp[n] and dentropy[n] (either may be NULL = 0) and the forward's stats and entropy; a
  * row whose target is outside [0, V) has none from dlogp.  The alternatives are not differentiated.
+ * A logit of -inf gets none, but for a target among them, which keeps its dlogp.
  * Rows of one call: fewer than 2^23 forward, 2^24 up to 32761 bf16 or 16381 fp32 words; backward fewer
  * than 2^24 pieces of 8185 bf16 or 4093 fp32 words. */
 typedef struct imgcap_logprob_desc {
