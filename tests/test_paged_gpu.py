@@ -1,6 +1,7 @@
 """Paged key/value cache: the planner, the writer and the attention of one new token per request,
 against plain implementations (the planner's request by request on the host, the attention's in 64
 bits), at the lengths, page sizes, strides and contents where they can go wrong."""
+import ctypes
 import math
 
 import pytest
@@ -16,6 +17,23 @@ BF, F = torch.bfloat16, torch.float32
 def _k():
     from imagecaptioningconvnext_amd import kernels
     return kernels
+
+
+def _abi():
+    from imagecaptioningconvnext_amd import _abi
+    return _abi
+
+
+def _desc(q, kc, width, max_len):
+    """The attention's descriptor, its sizes and types only, with addresses that are not read."""
+    d = _abi().PagedAttnDesc()
+    d.dtype, (d.B, d.H, d.dh), (d.pages, d.page, d.Hkv, _) = _k().dt(q), q.shape, kc.shape
+    d.width, d.max_len, d.scale = width, max_len, 1.0
+    d.q_row, d.q_head, d.o_row, d.o_head = q.stride(0), q.stride(1), q.stride(0), q.stride(1)
+    d.k_page, d.k_tok, d.k_head = d.v_page, d.v_tok, d.v_head = kc.stride()[:3]
+    d.table_row = width
+    d.q = d.k = d.v = d.o = d.table = d.lens = kc.data_ptr()
+    return d
 
 
 # ---- attention ------------------------------------------------------------------------------
@@ -256,6 +274,44 @@ def test_attention_far_offsets(hip_device, page):
     small = torch.searchsorted(used, table.clamp(min=0).long()).to(torch.int32)
     out, _, tol, _ = _reference(q, kc[used], vc[used], small, lens, dh ** -0.5)
     assert bool(((got.cpu().double() - out).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype,H,hkv,dh,n,parts", [
+    (BF, 8, 1, 64, 140001, 274), (F, 8, 1, 64, 140001, 274),     # joined by 32 columns, past 256 parts
+    (BF, 96, 1, 64, 70001, 137), (F, 96, 1, 64, 70001, 137),     # by whole rows of 64, past 128
+    (BF, 256, 2, 128, 35001, 69), (F, 256, 2, 128, 35001, 69),   # by whole rows of 128, past 64
+    (BF, 2, 1, 64, 600001, 987), (F, 3, 1, 128, 530003, 975),    # as many parts as there can be, or nearly
+])
+def test_attention_of_many_parts(hip_device, dtype, H, hkv, dh, n, parts):
+    """Lengths in more parts than the join takes in one round; the second row ends in its first part and
+    the third in the middle of one.  As in _reference, by products of whole matrices, but for the sums:
+    a term of a part of c tokens passes c / 16 additions in its lane, 32 in its workgroup, then an eighth
+    of the parts and 32 more in the join."""
+    K, dev = _k(), hip_device
+    g = torch.Generator(dev).manual_seed(41)
+    lens, page = [n, 77, n // 2 + 5], 256
+    width = (n + page - 1) // page
+    kc, vc = (torch.randn(width + 1, page, hkv, dh, generator=g, device=dev).to(dtype) for _ in range(2))
+    table = torch.stack([torch.randperm(width + 1, generator=g, device=dev)[:width] for _ in lens]).to(torch.int32)
+    q = torch.randn(3, H, dh, generator=g, device=dev).to(dtype)
+    d, need = _desc(q, kc, width, n), ctypes.c_int64(0)
+    assert _abi().lib().imgcap_paged_attention_ws(ctypes.byref(d), ctypes.byref(need)) == 0
+    assert need.value == 3 * H * parts * (dh + 2) * 4
+    lse = torch.empty(3, H, device=dev)
+    got = K.paged_attention(q, kc, vc, table, torch.tensor(lens, dtype=torch.int32, device=dev), max_len=n, lse=lse)
+    for b, m in enumerate(lens):
+        t = torch.arange(m, device=dev)
+        k, v = (c[table[b, t // page].long(), t % page].double().transpose(0, 1).contiguous() for c in (kc, vc))
+        x = q[b].double().view(hkv, H // hkv, dh)
+        s = torch.matmul(x, k.transpose(1, 2).contiguous()) * dh ** -0.5
+        E = torch.matmul(x.abs(), k.abs().transpose(1, 2).contiguous()).amax(-1).view(H) * dh ** -0.5
+        p = torch.softmax(s, -1)
+        out, room = (torch.matmul(p, w).view(H, dh) for w in (v, v.abs()))
+        w = 2 * ((dh + 4) * U * E + 2.0 ** -22) + (n / parts / 16 + parts / 8 + 64) * U
+        ref = torch.logsumexp(s, -1).view(H)
+        assert bool(((lse[b].double() - ref).abs() <= w + 4 * U * ref.abs()).all()), b
+        tol = (w + (2.0 ** -15 if dtype == BF else 0))[:, None] * room + HALF[dtype] * out.abs()
+        assert bool(((got[b].double() - out).abs() <= tol).all()), b
 
 
 @pytest.mark.parametrize("dtype", [BF, F])
