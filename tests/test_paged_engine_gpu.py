@@ -6,6 +6,7 @@ terms each, (128 + 2) 2^-24 = 8e-6 relative apiece at worst and random in sign, 
 below 1e-4 of the logits' norm (1.3e-4 if every one were at its worst and of one sign)."""
 import functools
 import json
+import math
 import os
 
 import pytest
@@ -283,3 +284,105 @@ def test_log_probs_are_those_of_the_predictions(hip_device):
     assert (logp.cpu().double() - want).abs().max() < 2e-6  # fp32 of values below 16: 4 half steps of 2^-21
     order = torch.sort(logits, dim=-1, descending=True, stable=True).indices[..., :5]
     assert torch.equal(ti.cpu(), order)
+
+
+def test_alternatives_are_the_best_words(hip_device):
+    """Every position's alternatives against the oracle's order: the same word wherever no other is within
+    the logits' error (1e-4 of a row's norm, at the top of this file), which most positions are, and one
+    of the same value within it everywhere."""
+    dec, p = _model(hip_device)
+    B, L, V, top = 4, 14, CFG["V"], 4
+    caps, lens = make_captions(B, L, [14, 9, 3, 12], V, 13)
+    enc = make_features((B, 7, 7, CFG["E"]), 14)
+    with torch.no_grad():
+        _, _, tl, ti = dec.logProbs(enc.to(hip_device), caps.to(hip_device), lens.to(hip_device), top=top)
+    logits = _oracle(p, enc, caps, lens)
+    best = logits.topk(top + 1, -1)
+    room = 1e-4 * logits.norm(dim=-1, keepdim=True)
+    ti = ti.cpu()
+    assert bool(((logits.gather(-1, ti) - best.values[..., :top]).abs() <= room).all())
+    assert all(len(set(r)) == top for r in ti.view(-1, top).tolist())
+    gaps = best.values[..., :-1] - best.values[..., 1:]
+    alone = (gaps > room) & torch.cat([torch.ones(B, L, 1, dtype=torch.bool), (gaps > room)[..., :-1]], -1)
+    assert alone.double().mean() > 0.75
+    assert torch.equal(ti[alone], best.indices[..., :top][alone])
+
+
+def _ending(eng, end, offset):
+    """Steps whose end word's logit is moved by offset(position)."""
+    step = eng.decode_step
+
+    def moved(st, ids):
+        t, logits = st["t"], step(st, ids)
+        logits[:, end] += offset(t)
+        return logits
+
+    eng.decode_step = moved
+
+
+def _plain_beam(p, enc, start, end, k, most, offset):
+    """Beam search that decodes every prefix again with the oracle: (words, the steps at which beams ended,
+    the least distance of a kept score to the next one)."""
+    rows, scores, done, ends, gap = [[start]], torch.zeros(1, dtype=torch.float64), [], [], math.inf
+    for t in range(most):
+        caps = torch.tensor(rows)
+        logits = _oracle(p, enc.expand(len(rows), -1, -1, -1), caps, torch.full((len(rows), 1), t + 2))[:, -1].clone()
+        logits[:, end] += offset(t)
+        best = torch.sort((scores[:, None] + torch.log_softmax(logits, -1)).view(-1), descending=True, stable=True)
+        gap = min(gap, (best.values[:k] - best.values[1:k + 1]).min().item())
+        new = [(rows[i // CFG["V"]] + [i % CFG["V"]], v) for i, v in zip(best.indices[:k].tolist(), best.values)]
+        done += [r for r in new if r[0][-1] == end]
+        ends += [t for r in new if r[0][-1] == end]
+        new = [r for r in new if r[0][-1] != end]
+        k = len(new)
+        if not k:
+            break
+        rows, scores = [r[0] for r in new], torch.stack([r[1] for r in new])
+    return max(done, key=lambda r: r[1])[0], ends, gap
+
+
+@pytest.mark.parametrize("k,seed,ends", [(3, 22, [72, 73, 73]), (4, 36, [71, 72, 72, 72])])
+def test_beam_search_past_64_positions(hip_device, k, seed, ends):
+    """Captions of more than 70 words: no beam may end before position 66, then they end one after another.
+    Scores closer than 5e-4, some thousand times their error in fp32, would not be a test of the search."""
+    from imagecaptioningconvnext_amd import beam
+    dec, p = _model(hip_device)
+    V, enc = CFG["V"], make_features((1, 7, 7, CFG["E"]), seed)
+
+    def offset(t):
+        return -1e4 if t < 66 else 0.02 * (t - 66) - 0.1
+
+    with torch.no_grad():
+        want, at, gap = _plain_beam(p, enc, V - 2, V - 1, k, 88, offset)
+    assert at == ends and gap > 5e-4
+    _ending(dec.engine(), V - 1, offset)
+    seq, _ = beam.caption_image_beam_search_transformer(_FixedEncoder(enc.to(hip_device)), dec,
+                                                        torch.zeros(3, 256, 256, dtype=torch.uint8), word_map(V),
+                                                        beamSize=k, max_decode_len=88)
+    assert seq == want
+
+
+def test_greedy_past_64_positions(hip_device):
+    """No row ends before position 66; from 70 on every row does.  Logits of every step against one pass of
+    the oracle over the words chosen, which are its best ones."""
+    dec, p = _model(hip_device)
+    B, L, V = 3, 80, CFG["V"]
+    enc = make_features((B, 7, 7, CFG["E"]), 37)
+
+    def offset(t):
+        return -1e4 if t < 66 else 0.0 if t < 70 else 1e4
+
+    _ending(dec.engine(), V - 1, offset)
+    preds, seqs = dec(teacherForcing=False, encoder_out=enc.to(hip_device), wordMap=word_map(V), maxDecodeLen=L)
+    preds, seqs = preds.cpu().double(), seqs.cpu()
+    caps = torch.cat([torch.full((B, 1), V - 2), seqs[:, :-1]], 1)
+    want = _oracle(p, enc, caps, torch.full((B, 1), L))
+    for b in range(B):
+        n = seqs[b].tolist().index(V - 1) + 1  # words with the end
+        assert 67 <= n <= 71
+        moved = want[b, :n] + torch.tensor([[offset(t) * (w == V - 1) for w in range(V)] for t in range(n)], dtype=torch.float64)
+        words = torch.arange(V) != V - 1
+        assert _rel(preds[b, :n][:, words], moved[:, words]) < 1e-4
+        room = 1e-4 * want[b, :n].norm(dim=-1)
+        assert bool((moved.gather(-1, seqs[b, :n, None])[:, 0] >= moved.amax(-1) - room).all())
+        assert bool((preds[b, n:] == 0).all())
