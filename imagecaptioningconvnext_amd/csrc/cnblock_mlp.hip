@@ -20,7 +20,7 @@
 namespace imgcap {
 
 #ifndef MLP_GELU
-#define MLP_GELU 2  // packed polynomial erf (|err| <= 1.5e-7, common.h gelu_fast2); 0 = libm erff
+#define MLP_GELU 2  // polynomial erf on two values at once (|err| <= 1.5e-7, common.h gelu_fast2); 0 = libm erff
 #endif
 #ifndef MLP_TAG
 #define MLP_TAG "erf"

@@ -362,7 +362,7 @@ __global__ __launch_bounds__(256) void dwconv7_ln_kernel(int B, int H, int W, in
 // The (TR+6) x (W+6) x 32 input patch (zero halo) is staged once into LDS with 16-byte
 // coalesced loads; each lane then slides a PW+6 register window along its row for each of
 // the 7 kernel rows (rows of another image than the lane's are skipped: image boundaries
-// inside a tile).  fp32 accumulation, packed two channels per FMA.
+// inside a tile).  fp32 accumulation, two channels at a time.
 // LDS layout: 16-byte slots; pixel px of patch row r at slot r*RS + 4*px + px/PW (one gap slot
 // after every PW pixels), slot s of the pixel = its channels 8s..8s+7 (fp32: two slots per 8
 // channels).  A wave reads slot wv of pixel g*PW + q across its lanes (row lr = lane / GW, group
@@ -470,7 +470,7 @@ __global__ __launch_bounds__(64 * DW_CT / NC) void dwconv7_kernel(int B, int H, 
   if (lr >= TR || orow >= R) return;
   const int h = (int)(orow % H);
   const int w0 = g * PW;
-  constexpr int NP = NC / 2;       // channel pairs per lane (packed fp32 FMAs)
+  constexpr int NP = NC / 2;       // channel pairs per lane
   f32x2 acc[PW][NP];
   {
     float b[NC];
@@ -899,8 +899,8 @@ void dw_roll_attr() {
 // is re-unpacked per kernel row (≈ 1.1 VALU per MAC).  Here a lane keeps its channel pair's 49
 // weight pairs in registers for the whole row, reads each of the 7 input rows once as coalesced
 // 4-byte bf16 pairs (64 lanes = 256 contiguous bytes, the next row requested before the current
-// one is used), unpacks it once and applies all 7 taps of that kernel row with packed FMAs
-// (≈ 0.7 VALU per MAC), and the grid is B*H rows x C/128 waves.  flip / res: the backward data gradient (taps mirrored, residual added), as dwconv7_kernel.
+// one is used), unpacks it once and applies all 7 taps of that kernel row (an FMA per MAC and the
+// unpacking), and the grid is B*H rows x C/128 waves.  flip / res: the backward data gradient (taps mirrored, residual added), as dwconv7_kernel.
 template <int W, bool LN, int R>
 __global__ __launch_bounds__(512) void dwconv7_cp_kernel(int H, int C, const bf16* __restrict__ x,
                                                          const float* __restrict__ w, const float* __restrict__ bias,

@@ -112,9 +112,9 @@ DEV void lp_join_lanes(float& c, float& s, float& t) {
 // there.  Where more than LP_CAND do (long ties), or too few (NaN), the alternatives are found one by
 // one, in passes over the row.
 // Bound by vector issue beside HBM: 8.4 instructions a logit (the exponential at a quarter of the rate)
-// and some 300 a wave.  MI355X: 3264 x 9490 bf16 with 5 alternatives 18.4 us (62 MB; 12.7 at the rate of
-// a large copy), 1000 x 131072 bf16 with 20 59.5 us (4.4 TB/s), 777 x 50257 fp32 with 10 35.8 us
-// (4.4 TB/s), 5 x 9490 fp32 6.1 us.
+// and some 300 a wave.  MI355X, calls one after another: 3264 x 9490 bf16 with 5 alternatives 17.0 us
+// (62 MB; 12.7 at the rate of a large copy), 1000 x 131072 bf16 with 20 58.4 us (4.5 TB/s), 777 x 50257
+// fp32 with 10 32.3 us (4.8 TB/s), 5 x 9490 fp32 5.5 us.
 template <typename T, int TPB, bool LONG>
 __global__ __launch_bounds__(TPB) void token_logprobs_kernel(int V, int top, const T* __restrict__ logits, long ld,
                                                              const int64_t* __restrict__ tgt, float* __restrict__ logp,
@@ -359,9 +359,9 @@ extern "C" int imgcap_token_logprobs(const imgcap_logprob_desc* d, void* stream)
                      (top == 0 || (d->top_logp && d->top_ids)),
                  "imgcap_token_logprobs: NULL operand");
   hipStream_t st = (hipStream_t)stream;
-  // Few rows: 1024 threads each, for latency (5 x 9490 6.1 us).  More than 512: 256 threads for rows that
-  // these hold in registers or nearly (3264 x 9490 22 us, 30 with 512), 512 beyond (1280 x 50257 fp32
-  // 50.4 us, 53.4 with 256; 1000 x 131072 bf16 61, 64 with 256).
+  // Few rows: 1024 threads each, for latency (5 x 9490 5.5 us).  More than 512: 256 threads for rows that
+  // these hold in registers or nearly (3264 x 9490 bf16 17.0 us, 24.0 with 512; 2000 x 9490 fp32 16.9,
+  // 18.0), 512 beyond (1280 x 50257 fp32 46.1 us, 50.1 with 256; 1000 x 131072 bf16 58.4, 60.8).
   const int vec = d->dtype == IMGCAP_BF16 ? 8 : 4, nvec = (V + 2 * vec - 2) / vec;
   const int tpb = n <= 512 ? 1024 : nvec <= 512 * 8 ? 256 : 512;
   IMGCAP_REQUIRE((int64_t)n * tpb < (1ll << 32), "imgcap_token_logprobs: too many rows for a launch (2^32 threads)");
