@@ -239,13 +239,6 @@ def fail(name, rc):
     raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
 
 
-def check(name, *args):
-    """Call an entry point that only computes on the host (no workspace is attached for it)."""
-    rc = getattr(lib(), name)(*args)
-    if rc != 0:
-        fail(name, rc)
-
-
 def call(name, *args):
     import torch
     dev = torch.cuda.current_device() if torch.cuda.is_available() else None
